@@ -65,7 +65,7 @@ def listed():
     ]
 
 
-MAX_PAIRS = 2 * 16 * 8192 * 2048 * 128     # scores times head size of the largest listed attention forward
+MAX_FLOPS = 2.4e11                         # of the largest listed case
 MAX_TRAIN = 2 * 16 * 4096 * 4096 * 128     # B * NH * T * T * D of the largest listed training step
 MAX_CACHE = 64 * 8192 * 4 * 128            # elements of the largest listed cache
 MAX_ROTARY = 16 * 4096 * 32 * 128
@@ -96,8 +96,11 @@ def draw(rng):
             while B == 1 and NH > NKV and NH * TK * TK * D > most:
                 NH -= NKV
         step = rng.choice([0, 1, 63, 64, 129]) if B > 1 else 0
-        return {"kind": kind, "B": B, "TQ": TQ, "TK": TK, "NH": NH, "NKV": NKV, "D": D, "window": window, "sinks": sinks,
+        case = {"kind": kind, "B": B, "TQ": TQ, "TK": TK, "NH": NH, "NKV": NKV, "D": D, "window": window, "sinks": sinks,
                 "step": step}
+        while work(case)["flops"] > MAX_FLOPS:
+            case["window"] //= 2
+        return case
     if kind in ("rotary", "rotary_back"):
         D = rng.choice([64, 128])
         NKV = rng.choice([1, 2, 3, 4, 8, 12])
