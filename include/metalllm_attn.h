@@ -70,8 +70,11 @@ enum {
   METALLLM_ATTN_E_ALIGN = -6,    /* a tensor pointer is not 16-byte aligned */
   METALLLM_ATTN_E_LAUNCH = -7,   /* the kernel launch failed */
   METALLLM_ATTN_E_LIBRARY = -8,  /* a platform library call (rocBLAS, device allocation) failed */
-  METALLLM_ATTN_E_CAPTURE = -9   /* per-device scratch would have to grow while the stream is being
+  METALLLM_ATTN_E_CAPTURE = -9,  /* per-device scratch would have to grow while the stream is being
                                     captured into a graph: call metalllmSublayerReserve first */
+  METALLLM_ATTN_E_WINDOW = -10,  /* window attention: window == 0, or more than 64 sinks */
+  METALLLM_ATTN_E_OVERLAP = -11  /* an output (or the workspace) shares memory with a buffer that the
+                                    call's description does not allow it to share */
 };
 
 /* Replaces the flashAttentionForward dispatch at model.h:459-473 (attention.metal:56-164).
@@ -349,6 +352,130 @@ int metalllmSublayerRoute(int phase, const metalllmSublayerBuffers* b, const Att
  * elements of the dQ split, floats of weight-gradient partials), and what metalllmSublayerReserve
  * sizes for p. Host-only. */
 int metalllmSublayerScratch(const AttentionParams* p, uint64_t need[2], uint64_t reserved[2]);
+
+/* ---- Window attention with sinks (no counterpart in the reference, whose attention is causal over all
+ * keys with as many key heads as query heads, attention.metal:56-299) ----
+ * Sequence b has lq query rows and lk keys: TQ and TK, or q_len[b] and k_len[b] where those device arrays
+ * (int32 [B], either may be NULL) are given; values outside 0..TQ, 0..TK are taken as the nearest of those.
+ * Query row i stands at position pos = lk - lq + i and sees key j where
+ *   j <= pos  and  (pos - j < window  or  j < sinks).
+ * TQ = TK without lengths is training or a whole prompt; TQ < TK a part of a prompt behind a cache; TQ = 1
+ * the next token. The NH / NKV query heads h in [n NH/NKV, (n + 1) NH/NKV) share key head n.
+ *
+ * q, out, dO, O, dQ: bf16 [B, TQ, NH, D]; k, v, dK, dV: bf16 [B, TK, NKV, D]; a head's D values beside each
+ * other, heads beside each other, rows and sequences at the strides below (elements, multiples of 8), so q, k
+ * and v may be slices of one buffer. dQ has q's strides, dK k's, dV v's, and dO and O out's. l, fp32
+ * [B, NH, TQ]: logsumexp of a row's visible scores q.k/sqrt(D).
+ * Rows i >= lq of out, l and dQ, and rows j >= lk of dK and dV, are left as they were, and what the inputs
+ * hold there, or in keys that no row sees, is never read into a result (it may be NaN); a key that only
+ * some rows see has no part in the others either. A row that sees nothing (lk < lq: pos < 0) gives out = 0,
+ * l = -inf, dQ = 0. Elsewhere NaN and infinities spread as the formulas have it.
+ * Scores, softmax statistics and sums are fp32; the softmax weights and dS are rounded to bf16 once each as
+ * matrix operands, the outputs once at the end. No atomics: results repeat bit for bit.
+ * Workspace: the size functions' bytes (0 possible for the forward: workspace may then be NULL), 16-byte
+ * aligned, no state between calls; it belongs to one call (or captured call's replay) at a time. The sizes
+ * depend on the params alone. Nothing is allocated and no memset is recorded: every call can be captured.
+ * Outputs and workspace must not share memory with inputs (METALLLM_ATTN_E_OVERLAP, judged from a tensor's
+ * first element to its last); dQ, dK and dV may be interleaved slices of one buffer.
+ * Validation: D in {64, 128}, NH a multiple of NKV, window >= 1, sinks <= 64, TQ, TK <= 2^24, row strides
+ * below 2^22, rows and sequences apart from each other, pointers 16-byte aligned (lengths 4). */
+typedef struct metalllmWindowParams {
+  uint32_t B, TQ, TK, NH, NKV, D;
+  uint32_t window; /* keys that a row sees up to its own; any value >= TK: all of them */
+  uint32_t sinks;  /* first keys that every row at or behind them sees */
+  uint64_t q_row, q_seq; /* elements from a token to the next, from a sequence to the next */
+  uint64_t k_row, k_seq;
+  uint64_t v_row, v_seq;
+  uint64_t o_row, o_seq;
+} metalllmWindowParams;
+
+int metalllmWindowForwardWorkspaceSize(const metalllmWindowParams* p, uint64_t* bytes);
+int metalllmWindowBackwardWorkspaceSize(const metalllmWindowParams* p, uint64_t* bytes);
+
+/* l may be NULL (serving). */
+int windowAttentionForward(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out, float* l,
+                           const int32_t* q_len, const int32_t* k_len, void* workspace, uint64_t workspace_bytes,
+                           const metalllmWindowParams* p, metalllm_stream_t stream);
+
+/* O and l are the forward's; dQ, dK, dV are written, not added to. */
+int windowAttentionBackward(const uint16_t* dO, const uint16_t* O, const float* l, const uint16_t* q, const uint16_t* k,
+                            const uint16_t* v, uint16_t* dQ, uint16_t* dK, uint16_t* dV, const int32_t* q_len,
+                            const int32_t* k_len, void* workspace, uint64_t workspace_bytes,
+                            const metalllmWindowParams* p, metalllm_stream_t stream);
+
+/* ---- Rotary positions (no counterpart in the reference, which adds a learned position to the embedding) ----
+ * Of a head's D values the first `dims` turn, in pairs (2i, 2i + 1) where interleaved, else (i, i + dims/2),
+ * i < dims/2, by angle = position * f_i radians; the others are copied. With c, s the angle's cosine and
+ * sine times `magnitude`: forward (x1, x2) -> (x1 c - x2 s, x1 s + x2 c), backward (the gradient)
+ * (x1 c + x2 s, x2 c - x1 s). f_i = base^(-2i/dims), scaled for contexts longer than trained on:
+ *   LINEAR  f_i / factor
+ *   PARTS   f_i keep + f_i / factor (1 - keep), keep = (turns - low) / (high - low) held in [0, 1], turns =
+ *           original * f_i / 2pi: pairs that turn often inside the original length keep their frequency
+ * The plan is host memory, filled once; calls copy it, so it need not outlive them. */
+#define METALLLM_ROTARY_PAIRS 128
+enum { METALLLM_ROTARY_PLAIN = 0, METALLLM_ROTARY_LINEAR = 1, METALLLM_ROTARY_PARTS = 2 };
+typedef struct metalllmRotaryScaling {
+  int32_t kind;
+  float magnitude;  /* factor on the turned values (1: none) */
+  double factor;    /* LINEAR, PARTS: > 0 */
+  double original;  /* PARTS: tokens of the original context */
+  double low, high; /* PARTS: turns, high > low */
+} metalllmRotaryScaling;
+typedef struct metalllmRotaryPlan {
+  double turns[METALLLM_ROTARY_PAIRS]; /* f_i / 2pi */
+  float magnitude;
+  uint32_t dims;
+  uint32_t interleaved;
+  uint32_t reserved;
+} metalllmRotaryPlan;
+typedef struct metalllmRotaryParams {
+  uint32_t B, T, NH, NKV, D;       /* D a multiple of 8, at most 256, dims <= D; NKV = 0: q alone, k NULL */
+  uint32_t reserved;
+  uint64_t q_row, q_seq, k_row, k_seq;     /* strides in elements, multiples of 8, as window attention's */
+  uint64_t qo_row, qo_seq, ko_row, ko_seq; /* of the outputs */
+} metalllmRotaryParams;
+
+/* scaling NULL: PLAIN, magnitude 1. dims even, at most 256, base > 0. */
+int metalllmRotaryPlanInit(uint32_t dims, double base, int interleaved, const metalllmRotaryScaling* scaling,
+                           metalllmRotaryPlan* plan);
+
+/* q: bf16 [B, T, NH, D], k: [B, T, NKV, D]; positions: device int32 [B, T] (any value; angles are reduced in 64
+ * bits), or NULL: token t at position t. q_out may be q and k_out k (with the same strides); otherwise
+ * outputs share no memory with inputs. Allocates nothing. */
+int rotaryForward(const uint16_t* q, const uint16_t* k, uint16_t* q_out, uint16_t* k_out, const int32_t* positions,
+                  const metalllmRotaryPlan* plan, const metalllmRotaryParams* p, metalllm_stream_t stream);
+int rotaryBackward(const uint16_t* dq, const uint16_t* dk, uint16_t* dq_out, uint16_t* dk_out, const int32_t* positions,
+                   const metalllmRotaryPlan* plan, const metalllmRotaryParams* p, metalllm_stream_t stream);
+
+/* ---- Root-mean-square norm with the residual's addition (beside layernormForward and residualAdd, which
+ * the reference has instead) ----
+ * Per row of x, residual (bf16 [rows, cols]): h = x + residual (fp32; residual NULL: h = x), sum = bf16(h)
+ * (required with a residual, else may be NULL), rstd = 1/sqrt(mean(h^2) + eps) (fp32 [rows], may be NULL),
+ * out = h rstd gamma (gamma bf16 [cols]), rounded once: to bf16, or by rmsnormForwardFp8 to e4m3 with fp32
+ * scales [rows, ceil(cols/group)] (group 0: one per row): scale = max |out| of the group / 448 (at least
+ * 2^-126; 1 for zeros), out8 = e4m3(out / scale).
+ * rmsnormBackward, h the stored sum: with xh = h rstd, g = dOut gamma: dX = bf16(dSum + rstd (g - xh mean(g xh)))
+ * (dSum, the gradient that reaches the sum from the residual stream, may be NULL: 0) is the gradient of x and
+ * of residual alike; dgamma[c] = sum over rows of dOut xh (fp32 [cols]), written, not added to. Sums in fp32 in a
+ * fixed order. Its workspace is as window attention's.
+ * sum and out (bf16) may each lie in x's or residual's memory, dX in dOut's, dSum's or h's; otherwise
+ * outputs are apart from inputs and each other. cols a multiple of 8, at most METALLLM_RMSNORM_MAX_COLS,
+ * rows below 2^31, group 0, 32, 64 or 128, pointers 16-byte aligned. Allocates nothing. */
+#define METALLLM_RMSNORM_MAX_COLS 8192
+typedef struct metalllmRmsnormParams {
+  uint32_t rows, cols;
+  float eps;
+  uint32_t group; /* rmsnormForwardFp8 alone */
+} metalllmRmsnormParams;
+
+int rmsnormForward(const uint16_t* x, const uint16_t* residual, uint16_t* sum, uint16_t* out, const uint16_t* gamma,
+                   float* rstd, const metalllmRmsnormParams* p, metalllm_stream_t stream);
+int rmsnormForwardFp8(const uint16_t* x, const uint16_t* residual, uint16_t* sum, uint8_t* out, float* scales,
+                      const uint16_t* gamma, float* rstd, const metalllmRmsnormParams* p, metalllm_stream_t stream);
+int metalllmRmsnormBackwardWorkspaceSize(const metalllmRmsnormParams* p, uint64_t* bytes);
+int rmsnormBackward(const uint16_t* dOut, const uint16_t* dSum, const uint16_t* h, const uint16_t* gamma, const float* rstd,
+                    uint16_t* dX, float* dgamma, void* workspace, uint64_t workspace_bytes,
+                    const metalllmRmsnormParams* p, metalllm_stream_t stream);
 
 /* Static description of an error code (no counterpart in the reference, which has no error
  * path per kernel; model.h:333-336,361-365 only print). */

@@ -9,8 +9,9 @@ from .attention import (AttentionError, AttentionParams, attention_backward, att
 
 from . import glue  # noqa: E402  (layernorm, residual add, dX cast around the sublayer)
 from . import sublayer  # noqa: E402  (the GEMMs around the attention core)
+from . import rmsnorm, rotary, window  # noqa: E402  (RMS norm with residual, rotary positions, window attention)
 
-__all__ = ["glue", "sublayer", "AttentionError", "AttentionParams", "attention_backward", "attention_forward", "backward_part",
+__all__ = ["glue", "rmsnorm", "rotary", "sublayer", "window", "AttentionError", "AttentionParams", "attention_backward", "attention_forward", "backward_part",
            "computeD", "flashAttentionBackward", "flashAttentionBackwardNoAlloc", "flashAttentionBackwardWorkspace",
            "flashAttentionForward", "forward_items", "library",
            "work_map", "workspace_bytes"]

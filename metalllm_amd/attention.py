@@ -22,7 +22,7 @@ LIB_PATH = os.path.join(PKG, "libmetalllm_attn.so")
 OK = 0
 ERRORS = {
     -1: "E_NULL", -2: "E_SEQLEN", -3: "E_HEADDIM", -4: "E_LAYOUT", -5: "E_SIZE", -6: "E_ALIGN", -7: "E_LAUNCH",
-    -8: "E_LIBRARY", -9: "E_CAPTURE",
+    -8: "E_LIBRARY", -9: "E_CAPTURE", -10: "E_WINDOW", -11: "E_OVERLAP",
 }
 EXPORTED = ("flashAttentionForward", "computeD", "flashAttentionBackward", "metalllmAttnBackwardPart",
             "metalllmAttnErrorString", "metalllmAttnWorkMap", "computeQKV", "projForward", "projBackwarddW",
@@ -31,7 +31,10 @@ EXPORTED = ("flashAttentionForward", "computeD", "flashAttentionBackward", "meta
             "layernormForward", "layernormBackward",
             "metalllmSublayerGraphCreate", "metalllmSublayerGraphLaunch", "metalllmSublayerGraphDestroy",
             "metalllmSublayerReserve", "flashAttentionBackwardNoAlloc", "metalllmAttnForwardItems",
-            "metalllmSublayerRoute", "metalllmAttnBackwardRoute", "metalllmSublayerScratch")
+            "metalllmSublayerRoute", "metalllmAttnBackwardRoute", "metalllmSublayerScratch",
+            "metalllmWindowForwardWorkspaceSize", "metalllmWindowBackwardWorkspaceSize", "windowAttentionForward",
+            "windowAttentionBackward", "metalllmRotaryPlanInit", "rotaryForward", "rotaryBackward", "rmsnormForward",
+            "rmsnormForwardFp8", "metalllmRmsnormBackwardWorkspaceSize", "rmsnormBackward")
 NOALLOC_SCRATCH_BYTES = 64 << 20  # METALLLM_ATTN_NOALLOC_SCRATCH_BYTES
 
 

@@ -17,7 +17,8 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libmetalllm_attn.so")
 SOURCES = ["attn_abi.hip", "attn_fwd.hip", "attn_bwd.hip", "attn_bwd_dq.hip", "attn_bwd_both.hip", "attn_bwd_dqs.hip", "attn_computed.hip",
-           "attn_noalloc.hip", "sublayer.hip", "sublayer_gemm.hip", "sublayer_tile.hip", "glue.hip"]
+           "attn_noalloc.hip", "sublayer.hip", "sublayer_gemm.hip", "sublayer_tile.hip", "glue.hip",
+           "attn_window_abi.hip", "attn_window_fwd.hip", "attn_window_token.hip", "attn_window_bwd.hip", "rotary.hip", "rmsnorm.hip"]
 LIBS = ["-L/opt/rocm/lib", "-lrocblas", "-Wl,-rpath,/opt/rocm/lib"]  # sublayer GEMMs
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -36,6 +37,8 @@ EXTRA = {
     "attn_bwd.hip": ["-mllvm", "-pragma-unroll-threshold=200000"],
     "attn_bwd_dq.hip": ["-mllvm", "-pragma-unroll-threshold=200000"],
     "attn_bwd_both.hip": ["-mllvm", "-pragma-unroll-threshold=200000"],
+    "attn_window_fwd.hip": ["-mllvm", "-pragma-unroll-threshold=200000"],
+    "attn_window_bwd.hip": ["-mllvm", "-pragma-unroll-threshold=200000"],
 }
 
 

@@ -163,6 +163,8 @@ const char* metalllmAttnErrorString(int code) {
     case METALLLM_ATTN_E_LAUNCH: return "kernel launch failed";
     case METALLLM_ATTN_E_LIBRARY: return "platform library call (rocBLAS, device allocation) failed";
     case METALLLM_ATTN_E_CAPTURE: return "scratch would grow during stream capture (call metalllmSublayerReserve first)";
+    case METALLLM_ATTN_E_WINDOW: return "window must be at least 1 and sinks at most 64";
+    case METALLLM_ATTN_E_OVERLAP: return "an output or the workspace shares memory that it must not share";
     default: return "unknown error";
   }
 }

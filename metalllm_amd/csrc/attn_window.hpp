@@ -1,0 +1,120 @@
+// attn_window.hpp -- attention over a window of keys with a few first keys that stay visible
+// (attn_window_*.hip): what the kernels share, and their launch interface. Shapes arrive validated.
+//
+// Sequence b has lq query rows and lk keys. Query row i stands at position pos = lk - lq + i, and sees
+// key j where j <= pos and (pos - j < window or j < sinks). Rows at a negative position see nothing.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "attn_launch.hpp"
+
+namespace mla {
+
+constexpr int kWinMaxSinks = 64;  // one key tile
+
+struct WinShape {
+  int B, TQ, TK, NH, NKV, G;  // G = NH / NKV query heads share a key head
+  int window, sinks;          // window at most 2^30
+  uint32_t q_row, k_row, v_row, o_row;  // elements from a token to the next
+  size_t q_seq, k_seq, v_seq, o_seq;    // elements from a sequence to the next
+  const int32_t* q_len;       // device [B], or NULL: TQ rows, TK keys each
+  const int32_t* k_len;
+  float scale;                // 1/sqrt(D)
+};
+
+struct WinFwdArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  uint16_t* out;
+  float* l;  // [B, NH, TQ], or NULL
+  WinShape s;
+  float* part;  // single-token form: partial results of the splits (win_token_floats)
+  int splits;
+};
+
+struct WinBwdArgs {
+  const uint16_t* dO;
+  const uint16_t* O;
+  const float* l;
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  uint16_t* dQ;
+  uint16_t* dK;
+  uint16_t* dV;
+  WinShape s;
+  float* Dsum;  // [B, NH, TQ] workspace: sum over d of dO * O
+  float* part;  // workspace: partial dK, dV of the sink keys, or NULL where nothing is split (splits = 0)
+  int splits;
+};
+
+// A sequence's lengths, held inside the buffers whatever the device arrays say.
+struct WinSeq {
+  int lq, lk, off;  // off = lk - lq: position of query row 0
+};
+__device__ __forceinline__ WinSeq win_seq(const WinShape& s, int b) {
+  int lq = s.q_len ? s.q_len[b] : s.TQ, lk = s.k_len ? s.k_len[b] : s.TK;
+  lq = min(max(lq, 0), s.TQ);
+  lk = min(max(lk, 0), s.TK);
+  return WinSeq{__builtin_amdgcn_readfirstlane(lq), __builtin_amdgcn_readfirstlane(lk),
+                __builtin_amdgcn_readfirstlane(lk - lq)};
+}
+
+// The 64-key tiles that query rows i0 .. i1 of a sequence (i1 < lq) visit, in order: the sink tile 0
+// alone where the window begins behind it, then the window's tiles t0 .. t1.
+struct WinTiles {
+  int t0, sink, n;  // first window tile, 1 where tile 0 comes before it, number of tiles
+  int lo, hi;       // rows of k and v that window tiles may read: every key outside is hidden from all
+  __device__ __forceinline__ int tile(int j) const { return j < sink ? 0 : t0 + j - sink; }
+};
+__device__ __forceinline__ WinTiles win_tiles(const WinShape& s, const WinSeq& q, int i0, int i1) {
+  WinTiles w{0, 0, 0, 0, 0};
+  const int last = q.off + i1;  // position of the last row
+  if (last < 0) return w;
+  const int first = max(0, q.off + i0 - s.window + 1);  // first key of the rows' windows
+  w.t0 = first / kTile;
+  w.sink = s.sinks > 0 && w.t0 > 0 ? 1 : 0;
+  w.n = last / kTile - w.t0 + 1 + w.sink;
+  w.lo = s.sinks > 0 && w.t0 == 0 ? 0 : first;
+  w.hi = last;
+  return w;
+}
+
+// Rows of one head as the query side of a workgroup or the key side of another see them.
+__device__ __forceinline__ int clamp_row(int r, int lo, int hi) { return min(max(r, lo), hi); }
+
+// Whether query position `pos` sees key j.
+__device__ __forceinline__ bool win_sees(const WinShape& s, int pos, int j) {
+  return j <= pos && (pos - j < s.window || j < s.sinks);
+}
+
+// ---- host ----
+// Rows of 16 (query row, head of the group) that the single-token form puts into one matrix product, and
+// the largest number of rows per key head that it takes.
+constexpr int kTokRows = 16;
+constexpr int kTokMost = 64;
+inline bool win_is_token(const WinShape& s) { return s.TQ * s.G <= kTokMost && s.TQ <= kTokRows; }
+int win_token_splits(const WinShape& s);
+inline size_t win_token_floats(const WinShape& s, int D, int splits) {
+  const size_t tiles = ((size_t)s.TQ * s.G + kTokRows - 1) / kTokRows;
+  return splits > 1 ? (size_t)s.B * s.NKV * tiles * splits * kTokRows * (D + 2) : 0;
+}
+// Parts that the query tiles beyond the window of the sink keys' block are dealt to (0: there are none).
+inline int win_sink_splits(const WinShape& s) {
+  const int64_t far = (int64_t)s.TK - (kBwdBlockN - 1) - s.window;  // rows that see the sinks alone of block 0
+  if (s.sinks == 0 || far <= 0) return 0;
+  const int64_t usual = ((int64_t)s.window + kBwdBlockN - 1) / kTile + 1, tiles = (far + kTile - 1) / kTile;
+  const int64_t n = (tiles + usual - 1) / usual;
+  return (int)(n < 64 ? n : 64);
+}
+inline size_t win_sink_floats(const WinShape& s, int D, int splits) {
+  return splits ? (size_t)s.B * s.NKV * (splits + 1) * 2 * kWinMaxSinks * D : 0;
+}
+
+hipError_t launch_window_forward(const WinFwdArgs& a, int D, hipStream_t s);
+hipError_t launch_window_token(const WinFwdArgs& a, int D, hipStream_t s);
+hipError_t launch_window_backward(const WinBwdArgs& a, int D, hipStream_t s);
+
+}  // namespace mla

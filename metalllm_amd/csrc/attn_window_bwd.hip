@@ -1,0 +1,720 @@
+// attn_window_bwd.hip -- windowAttentionBackward on gfx950.
+//
+// With s = q.k/sqrt(D), p = exp(s - l) over the visible keys (l the forward's logsumexp), Dl = sum_d dO.O,
+// dP = dO.v and dS = p (dP - Dl):  dV = P^T.dO,  dK = dS^T.q/sqrt(D),  dQ = dS.k/sqrt(D).
+// Products accumulate in fp32 over all tiles and are rounded once; p and dS are rounded to bf16, the type of
+// the matrix cores' operands (half a step of 2^-8 each, as of the outputs). No atomics: every output has
+// one owner, and the sum over the query heads of a key head runs in the owner, so results repeat bit for bit.
+//
+// Two kernels, then a small one where there are sinks:
+//   win_dq_kernel    query owner: 4 waves x 32 rows of a head, over the key tiles that they see
+//                    (attn_window_fwd.hip's order). Also writes Dl and l log2(e) of its rows for the next.
+//   win_dkdv_kernel  key owner: 4 waves x 32 keys of a key head, over the query tiles that see them, head
+//                    by head of the group. The sinks of block 0 are seen by every later row, so the query
+//                    tiles beyond the block's windows are dealt to workgroups of their own, which keep the
+//                    sums of the sink keys alone in fp32.
+//   win_sink_kernel  dK, dV of the sink keys from those parts, in order.
+// A tile that is seen in part is masked by one unsigned compare per score; in the key owner the
+// compare's limit belongs to the lane's key and covers window, sinks and the sequence's end.
+#include "attn_common.hpp"
+#include "attn_window.hpp"
+
+namespace mla {
+
+typedef __attribute__((address_space(3))) uint16_t lds_u16w;
+__device__ __forceinline__ uint32_t lds_at(const void* p) { return (uint32_t)(uintptr_t)(const lds_u16w*)p; }
+__device__ __forceinline__ u32x4 lds_b128_w(uint32_t a) {
+  return *(const __attribute__((address_space(3))) u32x4*)(uintptr_t)a;
+}
+__device__ __forceinline__ f32x4 lds_f4_w(uint32_t a) {
+  return *(const __attribute__((address_space(3))) f32x4*)(uintptr_t)a;
+}
+__device__ __forceinline__ u32x2 lds_tr_w(uint32_t a) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) i16x4*)(uintptr_t)a));
+}
+// Global -> LDS copy of 4 bytes per lane to m0 + 4 lane (untracked, as dma16)
+__device__ __forceinline__ void dma4_v(const void* src, uint32_t m0) {
+  asm volatile("global_load_lds_dword %0, off" ::"v"(src), "{m0}"(m0) : "memory");
+}
+// sum over 8 pairs of bf16 products, added to x
+__device__ __forceinline__ float dot8(u32x4 a, u32x4 b, float x) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    x = fmaf(bf_lo(a[w]), bf_lo(b[w]), x);
+    x = fmaf(bf_hi(a[w]), bf_hi(b[w]), x);
+  }
+  return x;
+}
+
+// Tiles of 64 rows of two tensors in LDS, padded: 16-byte row reads and transposing reads.
+template <int D>
+struct WbCfg {
+  static constexpr int P = D == 128 ? D + 24 : D + 8;
+  static constexpr int TBYTES = kTile * P * 2;
+  static constexpr int SLOTS = P / 8;
+  static constexpr int LPW = (SLOTS + 3) / 4;
+  static constexpr int STAT = 2 * TBYTES;  // key owner: l log2(e) and Dl of the tile's rows
+  static constexpr int STAGE = 2 * TBYTES + 512;
+  static constexpr int KC = D / 16;
+  static constexpr int DT = D / 32;
+};
+
+template <int V>
+struct IntTag {
+  static constexpr int value = V;
+};
+
+// ---- dQ: query owner ----
+
+template <int D>
+__global__ void __launch_bounds__(256, 2) win_dq_kernel(WinBwdArgs a) {
+  using C = WbCfg<D>;
+  constexpr int BM = kDqBlockM;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * C::TBYTES];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = lane >> 5, l32 = lane & 31;
+  const WinShape& s = a.s;
+  const int nqb = (s.TQ + BM - 1) / BM;
+  int group, blk;
+  decode_workgroup(blockIdx.x, s.B * s.NKV, nqb * s.G, true, kBwdDispatchRound, group, blk);
+  const int b = group / s.NKV, kvh = group - b * s.NKV;
+  const int qb = blk / s.G, head = kvh * s.G + (blk - qb * s.G);
+  const WinSeq sq = win_seq(s, b);
+  const int i0 = qb * BM;
+  if (i0 >= sq.lq) return;
+  const int i1 = min(i0 + BM, sq.lq) - 1;
+  const WinTiles wt = win_tiles(s, sq, i0, i1);
+  const int i = i0 + 32 * wave + l32, ic = min(i, i1);
+  const bool row_ok = i <= i1;
+  const int pos = sq.off + i;
+  uint16_t* dQg = a.dQ + b * s.q_seq + (size_t)ic * s.q_row + head * D;
+  const size_t stat = ((size_t)b * s.NH + head) * s.TQ + ic, stats = (size_t)s.B * s.NH * s.TQ;
+
+  // Q^T and dO^T as B operands: lane holds the row, d = 16c + 8h .. +7
+  u32x4 Qr[C::KC], Gr[C::KC];
+  const uint16_t* Qg = a.q + b * s.q_seq + (size_t)ic * s.q_row + head * D + 8 * h;
+  const size_t o_at = b * s.o_seq + (size_t)ic * s.o_row + head * D + 8 * h;
+  float dl = 0.0f;
+#pragma unroll
+  for (int c = 0; c < C::KC; ++c) {
+    Qr[c] = *(const u32x4*)(Qg + 16 * c);
+    Gr[c] = *(const u32x4*)(a.dO + o_at + 16 * c);
+    dl = dot8(Gr[c], *(const u32x4*)(a.O + o_at + 16 * c), dl);
+  }
+  dl = sum_halves(dl);
+  const float l2 = a.l[stat] * kLog2e;
+  if (row_ok && h == 0) {
+    a.Dsum[stat] = dl;
+    a.Dsum[stats + stat] = l2;
+  }
+  const float sl = s.scale * kLog2e;
+
+  const char* Kg = (const char*)(a.k + b * s.k_seq + kvh * D);
+  const char* Vg = (const char*)(a.v + b * s.v_seq + kvh * D);
+  const uint32_t krs = 2 * s.k_row, vrs = 2 * s.v_row;
+  int crow[C::LPW];
+  uint32_t cchunk[C::LPW];
+#pragma unroll
+  for (int j = 0; j < C::LPW; ++j) {
+    const int t = 64 * (wave + 4 * j) + lane;
+    crow[j] = t / C::SLOTS;
+    cchunk[j] = 16 * min(t % C::SLOTS, D / 8 - 1);
+  }
+  const uint32_t smem_a = lds_at(smem);
+  auto issue_tile = [&](int j) {
+    const int kt = wt.tile(j);
+    const bool sink_tile = j < wt.sink;
+    const int lo = sink_tile ? 0 : max(wt.lo - kt * kTile, 0);
+    const int hi = sink_tile ? s.sinks - 1 : min(wt.hi - kt * kTile, kTile - 1);
+    const char* ks = Kg + (size_t)kt * kTile * krs;
+    const char* vs = Vg + (size_t)kt * kTile * vrs;
+    const uint32_t dst = smem_a + (j & 1) * 2 * C::TBYTES;
+#pragma unroll
+    for (int n = 0; n < C::LPW; ++n)
+      if (wave + 4 * n < C::SLOTS) {
+        const int r = clamp_row(crow[n], lo, hi);
+        dma16(__umul24(r, krs) + cchunk[n], ks, dst + 1024 * (wave + 4 * n));
+        dma16(__umul24(r, vrs) + cchunk[n], vs, dst + C::TBYTES + 1024 * (wave + 4 * n));
+      }
+  };
+  const uint32_t row_rd = 2 * (l32 * C::P + 8 * h);
+  const int g16 = lane >> 4, s16 = lane & 15;
+  const uint32_t tr_rd = 2 * ((4 * h + (s16 >> 2)) * C::P + 16 * (g16 & 1) + 4 * (s16 & 3));
+
+  f32x16 dQa[C::DT];
+#pragma unroll
+  for (int t = 0; t < C::DT; ++t) dQa[t] = zero16();
+
+  // One key tile: the products in order, one per slot: S and dP of keys 0-31 in turn, of keys 32-63, then
+  // dQ by 16-key chunk; pair p of half t goes through its three stages (exponent; p and dP - Dl; dS packed)
+  // from slot enter(t, p) on, between products that do not need it. A dQ product comes after the slot
+  // that packs its chunk's last pair.
+  constexpr int PPS = D == 64 ? 2 : 1;
+  struct Sched {
+    static constexpr int enter(int t, int p) { return (t ? 4 * C::KC : 2 * C::KC) + p / PPS; }
+    static constexpr int dq_slot(int k) {
+      int slot = 4 * C::KC - 1;
+      for (int j = 0; j <= k; ++j) {
+        const int c = j / C::DT, ready = enter(c / 2, 4 * (c % 2) + 3) + 2;
+        slot = (slot + 1 > ready + 1) ? slot + 1 : ready + 1;
+      }
+      return slot;
+    }
+    static constexpr int product_at(int i) {
+      if (i < 4 * C::KC) return i;
+      for (int k = 0; k < 4 * C::DT; ++k)
+        if (dq_slot(k) == i) return 4 * C::KC + k;
+      return -1;
+    }
+  };
+  constexpr int NM = 4 * C::KC + 4 * C::DT, NV = Sched::dq_slot(4 * C::DT - 1) + 1;
+  auto tile = [&](int j, auto mask_tag) __attribute__((always_inline)) {
+    constexpr int MASK = decltype(mask_tag)::value;
+    const uint32_t kb = smem_a + (j & 1) * 2 * C::TBYTES, vb = kb + C::TBYTES;
+    int dq = 0, sq_ = 0;
+    if (MASK) {
+      const int kt = wt.tile(j);
+      dq = pos - kt * kTile - 4 * h;
+      asm volatile("" : "+v"(dq));
+      if (MASK == 2) sq_ = min(s.sinks - kt * kTile - 4 * h, dq + 1);
+    }
+    auto seen = [&](int off) {
+      return (uint32_t)(dq - off) < (uint32_t)s.window || (MASK == 2 && off < sq_);
+    };
+    f32x16 x0 = zero16(), x1 = zero16(), y0 = zero16(), y1 = zero16();
+    uint32_t dS[16];
+    constexpr int RING = 6;
+    auto ahead = [](int n) { return n < 2 * C::KC ? 5 : 2; };
+    u32x4 ring[RING];
+    auto op_of = [&](int n) -> u32x4 {
+      if (n < 4 * C::KC) {
+        const int t = n / (2 * C::KC), isdp = n & 1, c = (n % (2 * C::KC)) >> 1;
+        return lds_b128_w((isdp ? vb : kb) + row_rd + 2 * (32 * t * C::P + 16 * c));
+      }
+      const int k = n - 4 * C::KC, dt = k % C::DT, c = k / C::DT;
+      const u32x2 lo = lds_tr_w(kb + tr_rd + 2 * (16 * c * C::P + 32 * dt));
+      const u32x2 hi = lds_tr_w(kb + tr_rd + 2 * ((16 * c + 8) * C::P + 32 * dt));
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+#pragma unroll
+    for (int n = 0; n <= ahead(0); ++n) ring[n] = op_of(n);
+    float ta[16], tb[16], ya[16], yb[16];
+    auto stage = [&](int t, int p, int st) {
+      f32x16& x = t ? x1 : x0;
+      f32x16& y = t ? y1 : y0;
+      const int u = 8 * t + p, r = 2 * p;
+      if (st == 0) {
+        ta[u] = fmaf(x[r], sl, -l2);
+        tb[u] = fmaf(x[r + 1], sl, -l2);
+        pin(ta[u], tb[u]);
+      } else if (st == 1) {
+        ta[u] = exp2_hw(ta[u]);
+        tb[u] = exp2_hw(tb[u]);
+        ya[u] = y[r] - dl;
+        yb[u] = y[r + 1] - dl;
+        pin(ta[u], tb[u]);
+        pin(ya[u], yb[u]);
+      } else {
+        float d0 = ta[u] * ya[u], d1 = tb[u] * yb[u];
+        if (MASK) {
+          const int off = 32 * t + 8 * (r >> 2) + (r & 3);
+          d0 = seen(off) ? d0 : 0.0f;
+          d1 = seen(off + 1) ? d1 : 0.0f;
+        }
+        uint32_t pk = pack_bf16(d0, d1);
+        pin(pk);
+        dS[u] = pk;
+      }
+    };
+#pragma unroll
+    for (int slot = 0; slot < NV; ++slot) {
+      const int n = Sched::product_at(slot);
+      if (n >= 0) {
+#pragma unroll
+        for (int k = (n ? n - 1 + ahead(n - 1) : ahead(0)) + 1; k <= n + ahead(n) && k < NM; ++k)
+          ring[k % RING] = op_of(k);
+        const u32x4& op = ring[n % RING];
+        if (n < 4 * C::KC) {
+          const int t = n / (2 * C::KC), c = (n % (2 * C::KC)) >> 1;
+          if (n & 1) {
+            if (t) y1 = mfma(op, Gr[c], y1);
+            else y0 = mfma(op, Gr[c], y0);
+          } else {
+            if (t) x1 = mfma(op, Qr[c], x1);
+            else x0 = mfma(op, Qr[c], x0);
+          }
+        } else {
+          const int k = n - 4 * C::KC, dt = k % C::DT, c = k / C::DT;
+          dQa[dt] = mfma(op, u32x4{dS[4 * c], dS[4 * c + 1], dS[4 * c + 2], dS[4 * c + 3]}, dQa[dt]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+          const int st = slot - Sched::enter(t, p);
+          if (st >= 0 && st < 3) stage(t, p, st);
+        }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  if (wt.n) {
+    issue_tile(0);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    const int last = sq.off + i0 + BM - 1, j_of = wt.sink - wt.t0;
+    int f0 = max(1, (max(0, last - s.window + 1) + kTile - 1) / kTile + j_of);
+    int f1 = min(max(0, sq.off + i0 + 1) / kTile + j_of, wt.n);
+    if (f0 >= f1) f0 = f1 = wt.n;
+    auto run = [&](int j, auto tag) __attribute__((always_inline)) {
+      if (j + 1 < wt.n) issue_tile(j + 1);
+      tile(j, tag);
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+    };
+    run(0, IntTag<2>());
+    int j = 1;
+    for (; j < f0; ++j) run(j, IntTag<1>());
+    for (; j < f1; ++j) run(j, IntTag<0>());
+    for (; j < wt.n; ++j) run(j, IntTag<1>());
+  }
+
+  // a hidden key whose row is not finite has added 0 * NaN to the rows of its tile: such rows are summed
+  // again over the keys that they see
+  float bad = 0.0f;
+#pragma unroll
+  for (int t = 0; t < C::DT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) bad = fmaf(dQa[t][r], 0.0f, bad);
+  const bool again = row_ok && (pos < 0 || (dl - dl == 0.0f && l2 - l2 == 0.0f)) && sum_halves(bad) != 0.0f;
+  if (__any(again)) {
+    if (again) {
+#pragma unroll
+      for (int t = 0; t < C::DT; ++t) dQa[t] = zero16();
+      const int first = max(0, pos - s.window + 1), ns = min(s.sinks, first);
+      const int count = pos < 0 ? 0 : ns + pos + 1 - first;
+      for (int t = 0; t < count; ++t) {
+        const int key = t < ns ? t : first + t - ns;
+        const uint16_t* kr = (const uint16_t*)(Kg + (size_t)key * krs);
+        const uint16_t* vr = (const uint16_t*)(Vg + (size_t)key * vrs);
+        float x = 0.0f, y = 0.0f;
+#pragma unroll
+        for (int c = 0; c < C::KC; ++c) {
+          x = dot8(*(const u32x4*)(kr + 16 * c + 8 * h), Qr[c], x);
+          y = dot8(*(const u32x4*)(vr + 16 * c + 8 * h), Gr[c], y);
+        }
+        x = sum_halves(x);
+        y = sum_halves(y);
+        const float d = round_bf16(exp2_hw(fmaf(x, sl, -l2)) * (y - dl));
+#pragma unroll
+        for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const u32x2 kk = *(const u32x2*)(kr + 32 * dt + 8 * g + 4 * h);
+            dQa[dt][4 * g] = fmaf(d, bf_lo(kk[0]), dQa[dt][4 * g]);
+            dQa[dt][4 * g + 1] = fmaf(d, bf_hi(kk[0]), dQa[dt][4 * g + 1]);
+            dQa[dt][4 * g + 2] = fmaf(d, bf_lo(kk[1]), dQa[dt][4 * g + 2]);
+            dQa[dt][4 * g + 3] = fmaf(d, bf_hi(kk[1]), dQa[dt][4 * g + 3]);
+          }
+      }
+    }
+  }
+  if (!row_ok) return;
+#pragma unroll
+  for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x16& o = dQa[dt];
+      *(u32x2*)(dQg + 32 * dt + 8 * g + 4 * h) = u32x2{pack_bf16(o[4 * g] * s.scale, o[4 * g + 1] * s.scale),
+                                                       pack_bf16(o[4 * g + 2] * s.scale, o[4 * g + 3] * s.scale)};
+    }
+}
+
+// ---- dK, dV: key owner ----
+
+// The part of a wave: 32 keys of a key head, their K and V rows as B operands, dK^T and dV^T in fp32 (chain
+// n < DT: dV of d tile n, else dK of d tile n - DT), and a step over 64 query rows staged in LDS.
+template <int D>
+struct WinKeyWave {
+  using C = WbCfg<D>;
+  int h;
+  float sl;
+  uint32_t row_rd, tr_rd, st_rd;
+  u32x4 Kr[C::KC], Vr[C::KC];
+  f32x16 st[2 * C::DT];
+
+  __device__ __forceinline__ void init(int lane, float scale) {
+    h = lane >> 5;
+    sl = scale * kLog2e;
+    const int l32 = lane & 31, g16 = lane >> 4, s16 = lane & 15;
+    row_rd = 2 * (l32 * C::P + 8 * h);
+    tr_rd = 2 * ((4 * h + (s16 >> 2)) * C::P + 16 * (g16 & 1) + 4 * (s16 & 3));
+    st_rd = 16 * h;
+#pragma unroll
+    for (int n = 0; n < 2 * C::DT; ++n) st[n] = zero16();
+  }
+
+  // Query rows staged at LDS byte address stage_a; MASK: row r of the tile (position p0 + r) sees the lane's
+  // key where (uint)(p0 + r - key) < lim; d0 = p0 + 4h - key. Slots (one product each):
+  //   [0, KC) S of rows 0-31  [KC, 2KC) dP  [2KC, 3KC) S of rows 32-63  [3KC, 4KC) dP  then 4 per chain
+  template <bool MASK>
+  __device__ __forceinline__ void step(uint32_t stage_a, int d0, uint32_t lim) {
+    constexpr int NS = 4 * C::KC + 8 * C::DT;
+    constexpr int PPS = 8 / C::KC;
+    uint32_t row_a = stage_a + row_rd, tr_a = stage_a + tr_rd, stat_a = stage_a + C::STAT + st_rd;
+    pin(row_a);
+    pin(tr_a);
+    pin(stat_a);
+    if (MASK) asm volatile("" : "+v"(d0));
+    f32x16 x0 = zero16(), x1 = zero16(), y0 = zero16(), y1 = zero16();
+    uint32_t Pp[16], dS[16];
+    auto operand = [&](int i) -> u32x4 {
+      if (i < 4 * C::KC) {
+        const int seg = i / C::KC, t = seg >> 1, c = i % C::KC;
+        return lds_b128_w(row_a + ((seg & 1) ? C::TBYTES : 0) + 2 * (32 * t * C::P + 16 * c));
+      }
+      const int k = i - 4 * C::KC, n = k / 4, j = k % 4, dt = n % C::DT;
+      const uint32_t src = tr_a + (n >= C::DT ? 0 : C::TBYTES) + 2 * (16 * j * C::P + 32 * dt);
+      const u32x2 lo = lds_tr_w(src), hi = lds_tr_w(src + 2 * 8 * C::P);
+      return u32x4{lo[0], lo[1], hi[0], hi[1]};
+    };
+    struct Work {
+      int kind, t, u0, cnt;
+    };
+    // pairs of vector work in slot i: kind 1 = p of half t, 2 = dS of half t
+    auto work = [&](int i) -> Work {
+      if (i < 4 * C::KC) {
+        const int seg = i / C::KC, u0 = (i % C::KC) * PPS;
+        if (seg == 1) return {1, 0, u0, PPS};
+        if (seg == 2) return {2, 0, u0, PPS};
+        if (seg == 3) return {1, 1, u0, PPS};
+        return {0, 0, 0, 0};
+      }
+      const int k = i - 4 * C::KC;
+      if (k < 4 * C::DT) {
+        constexpr int SPAN = (4 * C::DT) / 8;
+        if (k % SPAN == 0) return {2, 1, k / SPAN, 1};
+      }
+      return {0, 0, 0, 0};
+    };
+    auto stats = [&](int i) -> f32x4 {
+      const Work w = work(i);
+      const uint32_t ad = stat_a + (w.kind == 2 ? 256 : 0) + 4 * (32 * w.t + 8 * (w.u0 >> 1) + 2 * (w.u0 & 1));
+      if (w.cnt == 2) return lds_f4_w(ad);
+      const f32x2 v = *(const __attribute__((address_space(3))) f32x2*)(uintptr_t)ad;
+      return f32x4{v[0], v[1], 0.0f, 0.0f};
+    };
+    auto seen = [&](int t, int r) { return (uint32_t)(d0 + 32 * t + 8 * (r >> 2) + (r & 3)) < lim; };
+    auto p_pair = [&](f32x16& x, int t, int u, float l0, float l1) {
+      const int r = 2 * u;
+      float p0 = exp2_hw(fmaf(x[r], sl, -l0));
+      float p1 = exp2_hw(fmaf(x[r + 1], sl, -l1));
+      if (MASK) {
+        p0 = seen(t, r) ? p0 : 0.0f;
+        p1 = seen(t, r + 1) ? p1 : 0.0f;
+      }
+      pin(p0, p1);
+      x[r] = p0;
+      x[r + 1] = p1;
+      uint32_t pk = pack_bf16(p0, p1);
+      pin(pk);
+      Pp[8 * t + u] = pk;
+    };
+    auto ds_pair = [&](const f32x16& x, const f32x16& y, int t, int u, float l0, float l1) {
+      const int r = 2 * u;
+      float e0 = x[r] * (y[r] - l0), e1 = x[r + 1] * (y[r + 1] - l1);
+      if (MASK) {  // a hidden row's dP or Dl may not be finite
+        e0 = seen(t, r) ? e0 : 0.0f;
+        e1 = seen(t, r + 1) ? e1 : 0.0f;
+      }
+      uint32_t pk = pack_bf16(e0, e1);
+      pin(pk);
+      dS[8 * t + u] = pk;
+    };
+    constexpr int RING = 5;
+    constexpr int SA = 2;
+    auto ahead = [](int i) { return i < C::KC ? 4 : 2; };
+    u32x4 ring[RING];
+    f32x4 sring[SA + 1];
+#pragma unroll
+    for (int k = 0; k <= ahead(0); ++k) ring[k] = operand(k);
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+#pragma unroll
+      for (int k = (i ? i - 1 + ahead(i - 1) : ahead(0)) + 1; k <= i + ahead(i) && k < NS; ++k)
+        ring[k % RING] = operand(k);
+      if (i + SA < NS && work(i + SA).kind) sring[(i + SA) % (SA + 1)] = stats(i + SA);
+      const u32x4& op = ring[i % RING];
+      if (i < 4 * C::KC) {
+        const int seg = i / C::KC, c = i % C::KC;
+        if (seg == 0) x0 = mfma(op, Kr[c], x0);
+        else if (seg == 1) y0 = mfma(op, Vr[c], y0);
+        else if (seg == 2) x1 = mfma(op, Kr[c], x1);
+        else y1 = mfma(op, Vr[c], y1);
+      } else {
+        const int k = i - 4 * C::KC, n = k / 4, j = k % 4;
+        const uint32_t* src = n >= C::DT ? dS : Pp;
+        st[n] = mfma(op, u32x4{src[4 * j], src[4 * j + 1], src[4 * j + 2], src[4 * j + 3]}, st[n]);
+      }
+      const Work w = work(i);
+      if (w.cnt) {
+        const f32x4 sv = sring[i % (SA + 1)];
+#pragma unroll
+        for (int v = 0; v < w.cnt; ++v) {
+          if (w.kind == 1)
+            p_pair(w.t ? x1 : x0, w.t, w.u0 + v, sv[2 * v], sv[2 * v + 1]);
+          else
+            ds_pair(w.t ? x1 : x0, w.t ? y1 : y0, w.t, w.u0 + v, sv[2 * v], sv[2 * v + 1]);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+};
+
+template <int D>
+__global__ void __launch_bounds__(256, D == 64 ? 2 : 1) win_dkdv_kernel(WinBwdArgs a) {
+  using C = WbCfg<D>;
+  constexpr int BN = kBwdBlockN;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * C::STAGE];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int h = lane >> 5, l32 = lane & 31;
+  const WinShape& s = a.s;
+  const int nkb = (s.TK + BN - 1) / BN;
+  int group, blk;
+  decode_workgroup(blockIdx.x, s.B * s.NKV, nkb + a.splits, false, kBwdDispatchRound, group, blk);
+  const int b = group / s.NKV, kvh = group - b * s.NKV;
+  const bool far = blk < a.splits;  // a part of the rows that see block 0's sinks alone
+  const int kb = far ? 0 : blk - a.splits;
+  const WinSeq sq = win_seq(s, b);
+  const int k0 = kb * BN;
+  const bool split = kb == 0 && a.splits > 0;  // sink keys go through the workspace
+  if (k0 >= sq.lk) return;                     // (the sink kernel reads nothing of such a sequence either)
+  const int k1 = min(k0 + BN, sq.lk) - 1;
+
+  // query rows [ilo, ihi] of each head, tiles [tlo, tlo + nt), and the items [f0, f1) of head * nt + tile
+  int ilo = max(0, k0 - sq.off);
+  int ihi = min(sq.lq - 1, min(k1 + s.window - 1, sq.lk - 1) - sq.off);
+  int tlo = 0, nt = 0;
+  if (ilo <= ihi) {
+    tlo = ilo / kTile;
+    nt = ihi / kTile - tlo + 1;
+  }
+  if (split) {
+    const int tn = ihi >= ilo ? tlo + nt : 0;  // the first tile that only sink keys are seen from
+    if (far) {
+      ilo = tn * kTile;
+      ihi = sq.lq - 1;
+      tlo = tn;
+      nt = max(0, (sq.lq + kTile - 1) / kTile - tn);
+    } else if (nt) {
+      ihi = min(sq.lq - 1, tn * kTile - 1);  // the rest of the last tile sees the sinks
+    }
+  }
+  const int items = s.G * nt;
+  const int f0 = far ? (int)((int64_t)items * blk / a.splits) : 0;
+  const int f1 = far ? (int)((int64_t)items * (blk + 1) / a.splits) : items;
+
+  const int key = k0 + 32 * wave + l32;
+  const bool sink_key = key < s.sinks;
+  const int most = sq.lk - key;  // rows of the sequence that stand at the key or behind it
+  const uint32_t lim = (uint32_t)max(0, sink_key ? most : far ? 0 : min(s.window, most));
+  const bool wave_on = far ? 32 * wave < s.sinks : k0 + 32 * wave <= k1;
+
+  const char* Qg = (const char*)(a.q + b * s.q_seq + kvh * s.G * D);
+  const char* Gg = (const char*)(a.dO + b * s.o_seq + kvh * s.G * D);
+  const size_t stat0 = ((size_t)b * s.NH + kvh * s.G) * s.TQ, stats = (size_t)s.B * s.NH * s.TQ;
+  const uint32_t qrs = 2 * s.q_row, grs = 2 * s.o_row;
+
+  WinKeyWave<D> wv;
+  wv.init(lane, s.scale);
+  {
+    const int kc = min(key, k1);  // rows past the end are read in bounds, never stored
+    const uint16_t* kr = a.k + b * s.k_seq + (size_t)kc * s.k_row + kvh * D + 8 * h;
+    const uint16_t* vr = a.v + b * s.v_seq + (size_t)kc * s.v_row + kvh * D + 8 * h;
+#pragma unroll
+    for (int c = 0; c < C::KC; ++c) {
+      wv.Kr[c] = *(const u32x4*)(kr + 16 * c);
+      wv.Vr[c] = *(const u32x4*)(vr + 16 * c);
+    }
+  }
+  int crow[C::LPW];
+  uint32_t cchunk[C::LPW];
+#pragma unroll
+  for (int j = 0; j < C::LPW; ++j) {
+    const int t = 64 * (wave + 4 * j) + lane;
+    crow[j] = t / C::SLOTS;
+    cchunk[j] = 16 * min(t % C::SLOTS, D / 8 - 1);
+  }
+  const uint32_t smem_a = lds_at(smem);
+  auto issue_tile = [&](int g, int t, int stage) {
+    const int lo = max(ilo - t * kTile, 0), hi = min(ihi - t * kTile, kTile - 1);
+    const char* qs = Qg + (size_t)t * kTile * qrs + 2 * g * D;
+    const char* gs = Gg + (size_t)t * kTile * grs + 2 * g * D;
+    const uint32_t dst = smem_a + stage * C::STAGE;
+#pragma unroll
+    for (int n = 0; n < C::LPW; ++n)
+      if (wave + 4 * n < C::SLOTS) {
+        const int r = clamp_row(crow[n], lo, hi);
+        dma16(__umul24(r, qrs) + cchunk[n], qs, dst + 1024 * (wave + 4 * n));
+        dma16(__umul24(r, grs) + cchunk[n], gs, dst + C::TBYTES + 1024 * (wave + 4 * n));
+      }
+    if (wave == 0) {
+      const float* p = a.Dsum + stat0 + (size_t)g * s.TQ + t * kTile + clamp_row(lane, lo, hi);
+      dma4_v(p + stats, dst + C::STAT);
+      dma4_v(p, dst + C::STAT + 256);
+    }
+  };
+  // tiles that every key of the block is seen from (far: the sink keys), without a row past the end
+  auto whole = [&](int t) {
+    const int p0 = sq.off + t * kTile;
+    return t * kTile + kTile <= sq.lq && (far || (p0 >= k0 + BN - 1 && p0 + kTile - 1 - k0 < s.window));
+  };
+
+  if (f0 < f1) {
+    int g = f0 / nt, t = tlo + f0 - g * nt;
+    issue_tile(g, t, 0);
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    for (int f = f0; f < f1; ++f) {
+      int gn = g, tn = t + 1;
+      if (tn == tlo + nt) {
+        tn = tlo;
+        ++gn;
+      }
+      if (f + 1 < f1) issue_tile(gn, tn, (f + 1 - f0) & 1);
+      const uint32_t st_a = smem_a + ((f - f0) & 1) * C::STAGE;
+      if (wave_on) {
+        if (whole(t))
+          wv.template step<false>(st_a, 0, 0);
+        else
+          wv.template step<true>(st_a, sq.off + t * kTile + 4 * h - key, lim);
+      }
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+      g = gn;
+      t = tn;
+    }
+  }
+
+  if (!wave_on) return;
+  // A row that does not see a key but shares its tile adds 0 * NaN to it where q or dO is not finite: such
+  // keys are summed again over the rows that see them.
+  float bad = 0.0f;
+#pragma unroll
+  for (int n = 0; n < 2 * C::DT; ++n)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) bad = fmaf(wv.st[n][r], 0.0f, bad);
+  const bool again = key <= k1 && (!far || sink_key) && sum_halves(bad) != 0.0f;
+  if (__any(again)) {
+    if (again) {
+#pragma unroll
+      for (int n = 0; n < 2 * C::DT; ++n) wv.st[n] = zero16();
+      for (int f = f0; f < f1; ++f) {
+        const int g = f / nt, t = tlo + f - g * nt;
+        const int ra = max(ilo, t * kTile), rb = min(ihi, t * kTile + kTile - 1);
+        for (int i = ra; i <= rb; ++i) {
+          if ((uint32_t)(sq.off + i - key) >= lim) continue;
+          const uint16_t* qr = (const uint16_t*)(Qg + (size_t)i * qrs) + g * D;
+          const uint16_t* gr = (const uint16_t*)(Gg + (size_t)i * grs) + g * D;
+          float x = 0.0f, y = 0.0f;
+#pragma unroll
+          for (int c = 0; c < C::KC; ++c) {
+            x = dot8(*(const u32x4*)(qr + 16 * c + 8 * h), wv.Kr[c], x);
+            y = dot8(*(const u32x4*)(gr + 16 * c + 8 * h), wv.Vr[c], y);
+          }
+          x = sum_halves(x);
+          y = sum_halves(y);
+          const float* sp = a.Dsum + stat0 + (size_t)g * s.TQ + i;
+          const float p = exp2_hw(fmaf(x, wv.sl, -sp[stats]));
+          const float d = round_bf16(p * (y - sp[0])), pr = round_bf16(p);
+#pragma unroll
+          for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const u32x2 qq = *(const u32x2*)(qr + 32 * dt + 8 * u + 4 * h);
+              const u32x2 gg = *(const u32x2*)(gr + 32 * dt + 8 * u + 4 * h);
+              f32x16& v = wv.st[dt];
+              f32x16& k = wv.st[C::DT + dt];
+              v[4 * u] = fmaf(pr, bf_lo(gg[0]), v[4 * u]);
+              v[4 * u + 1] = fmaf(pr, bf_hi(gg[0]), v[4 * u + 1]);
+              v[4 * u + 2] = fmaf(pr, bf_lo(gg[1]), v[4 * u + 2]);
+              v[4 * u + 3] = fmaf(pr, bf_hi(gg[1]), v[4 * u + 3]);
+              k[4 * u] = fmaf(d, bf_lo(qq[0]), k[4 * u]);
+              k[4 * u + 1] = fmaf(d, bf_hi(qq[0]), k[4 * u + 1]);
+              k[4 * u + 2] = fmaf(d, bf_lo(qq[1]), k[4 * u + 2]);
+              k[4 * u + 3] = fmaf(d, bf_hi(qq[1]), k[4 * u + 3]);
+            }
+        }
+      }
+    }
+  }
+  if (key > k1) return;
+  if (split && sink_key) {  // part 0: the block's own rows, then the far parts; fp32 [dK, dV][64][D]
+    float* out = a.part + ((size_t)group * (a.splits + 1) + (far ? blk + 1 : 0)) * 2 * kWinMaxSinks * D + key * D;
+#pragma unroll
+    for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const f32x16& v = wv.st[dt];
+        const f32x16& k = wv.st[C::DT + dt];
+        const int d0 = 32 * dt + 8 * u + 4 * h;
+        *(f32x4*)(out + d0) = f32x4{k[4 * u], k[4 * u + 1], k[4 * u + 2], k[4 * u + 3]};
+        *(f32x4*)(out + kWinMaxSinks * D + d0) = f32x4{v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]};
+      }
+    return;
+  }
+  if (far) return;
+  uint16_t* dKg = a.dK + b * s.k_seq + (size_t)key * s.k_row + kvh * D;
+  uint16_t* dVg = a.dV + b * s.v_seq + (size_t)key * s.v_row + kvh * D;
+#pragma unroll
+  for (int dt = 0; dt < C::DT; ++dt)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const f32x16& v = wv.st[dt];
+      const f32x16& k = wv.st[C::DT + dt];
+      const int d0 = 32 * dt + 8 * u + 4 * h;
+      *(u32x2*)(dKg + d0) = u32x2{pack_bf16(k[4 * u] * s.scale, k[4 * u + 1] * s.scale),
+                                  pack_bf16(k[4 * u + 2] * s.scale, k[4 * u + 3] * s.scale)};
+      *(u32x2*)(dVg + d0) = u32x2{pack_bf16(v[4 * u], v[4 * u + 1]), pack_bf16(v[4 * u + 2], v[4 * u + 3])};
+    }
+}
+
+// dK, dV of the sink keys: one workgroup per (sequence, key head), a thread per four columns of a row.
+template <int D>
+__global__ void __launch_bounds__(256) win_sink_kernel(WinBwdArgs a) {
+  const WinShape& s = a.s;
+  const int group = blockIdx.x, b = group / s.NKV, kvh = group - b * s.NKV;
+  const int keys = min(s.sinks, win_seq(s, b).lk);
+  const float* in = a.part + (size_t)group * (a.splits + 1) * 2 * kWinMaxSinks * D;
+  for (int t = threadIdx.x; t < 2 * keys * (D / 4); t += 256) {
+    const int c = t % (D / 4), r = t / (D / 4), key = r >> 1, isv = r & 1;
+    const float* p = in + (size_t)isv * kWinMaxSinks * D + key * D + 4 * c;
+    f32x4 sum = *(const f32x4*)p;
+    for (int v = 1; v <= a.splits; ++v) sum += *(const f32x4*)(p + (size_t)v * 2 * kWinMaxSinks * D);
+    if (!isv) sum *= s.scale;
+    uint16_t* o = isv ? a.dV + b * s.v_seq + (size_t)key * s.v_row : a.dK + b * s.k_seq + (size_t)key * s.k_row;
+    *(u32x2*)(o + kvh * D + 4 * c) = u32x2{pack_bf16(sum[0], sum[1]), pack_bf16(sum[2], sum[3])};
+  }
+}
+
+hipError_t launch_window_backward(const WinBwdArgs& a, int D, hipStream_t s) {
+  const WinShape& p = a.s;
+  const unsigned groups = (unsigned)(p.B * p.NKV);
+  const unsigned nq = groups * p.G * ((p.TQ + kDqBlockM - 1) / kDqBlockM);
+  const unsigned nk = groups * ((p.TK + kBwdBlockN - 1) / kBwdBlockN + a.splits);
+  hipLaunchKernelGGL((D == 64 ? win_dq_kernel<64> : win_dq_kernel<128>), dim3(nq), dim3(256), 0, s, a);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((D == 64 ? win_dkdv_kernel<64> : win_dkdv_kernel<128>), dim3(nk), dim3(256), 0, s, a);
+  e = hipGetLastError();
+  if (e != hipSuccess || a.splits == 0) return e;
+  hipLaunchKernelGGL((D == 64 ? win_sink_kernel<64> : win_sink_kernel<128>), dim3(groups), dim3(256), 0, s, a);
+  return hipGetLastError();
+}
+
+}  // namespace mla

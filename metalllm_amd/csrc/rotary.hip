@@ -1,0 +1,235 @@
+// rotary.hip -- rotary positions of q and k (include/metalllm_attn.h), HBM-bound.
+//
+// Pair i of a token at position pos turns by pos * f_i. The plan holds f_i / 2pi in 64 bits: the angle in
+// turns is pos * f_i, reduced to [-1/2, 1/2] in 64 bits (at position 10^6 a 32-bit product would be off by
+// 2^-5 of a turn for the fastest pair) and only then rounded to 32, where v_sin_f32 and v_cos_f32 take
+// turns. A thread owns 8 pairs of a token: it computes their sines once, then turns them in kHeads heads,
+// q and k in one launch. Halves of 8 pairs that are no whole 16-byte chunks go element by element.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/metalllm_attn.h"
+#include "overlap.hpp"
+
+namespace {
+
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+struct RotArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  uint16_t* qo;
+  uint16_t* ko;
+  const int32_t* pos;
+  metalllmRotaryParams p;
+  metalllmRotaryPlan plan;
+};
+
+__device__ __forceinline__ uint32_t pk(float lo, float hi) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{lo, hi}, b2));
+}
+__device__ __forceinline__ float lo_f(uint32_t x) { return __uint_as_float(x << 16); }
+__device__ __forceinline__ float hi_f(uint32_t x) { return __uint_as_float(x & 0xffff0000u); }
+
+constexpr int kHeads = 4;  // heads per thread: the sines of 8 pairs cost about as much as turning two heads
+
+// VEC: R is a multiple of 16, so a chunk's 8 pairs are two 16-byte chunks of the head in either order.
+// Chunks R/16 .. of a head (the part that does not turn) are copied, 16 values each.
+template <bool VEC>
+__global__ void __launch_bounds__(256) rotary_kernel(RotArgs a, int back, uint32_t chunks, uint32_t parts, uint32_t work) {
+  const uint32_t id = blockIdx.x * 256u + threadIdx.x;
+  if (id >= work) return;
+  const uint32_t rest = id / chunks, c = id - rest * chunks;
+  const uint32_t token = rest / parts, part = rest - token * parts;
+  const uint32_t b = token / a.p.T, t = token - b * a.p.T;
+  const uint32_t R = a.plan.dims, half = R / 2, turning = (half + 7) / 8;
+  const uint32_t h0 = part * kHeads, h1 = min(h0 + kHeads, a.p.NH + a.p.NKV);
+  const uint16_t* q = a.q + b * a.p.q_seq + t * a.p.q_row;
+  const uint16_t* k = a.k + b * a.p.k_seq + t * a.p.k_row;
+  uint16_t* qo = a.qo + b * a.p.qo_seq + t * a.p.qo_row;
+  uint16_t* ko = a.ko + b * a.p.ko_seq + t * a.p.ko_row;
+
+  if (c >= turning) {  // the part of the head behind the first R: values R + 16 (c - turning) ..
+    const uint32_t d0 = R + 16 * (c - turning), d1 = min(d0 + 16, a.p.D);
+    for (uint32_t h = h0; h < h1; ++h) {
+      const bool isq = h < a.p.NH;
+      const uint16_t* x = isq ? q + h * a.p.D : k + (h - a.p.NH) * a.p.D;
+      uint16_t* y = isq ? qo + h * a.p.D : ko + (h - a.p.NH) * a.p.D;
+      if (x == y) continue;
+      if (VEC) {  // R, hence d0, is a multiple of 16, D of 8
+        *(u4*)(y + d0) = *(const u4*)(x + d0);
+        if (d0 + 8 < d1) *(u4*)(y + d0 + 8) = *(const u4*)(x + d0 + 8);
+      } else {
+        for (uint32_t d = d0; d < d1; ++d) y[d] = x[d];
+      }
+    }
+    return;
+  }
+  const double pos = a.pos ? (double)a.pos[token] : (double)t;
+  float cs[8], sn[8];
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const uint32_t i = min(8 * c + u, half - 1);
+    double turn = pos * a.plan.turns[i];
+    turn -= rint(turn);
+    const float f = (float)turn;
+    cs[u] = __builtin_amdgcn_cosf(f) * a.plan.magnitude;
+    sn[u] = __builtin_amdgcn_sinf(f) * a.plan.magnitude;
+    if (back) sn[u] = -sn[u];
+  }
+  const bool inter = a.plan.interleaved != 0;
+  if (VEC) {
+    // two 16-byte chunks of a head: values 16c .. 16c + 15 (neighbours paired) or 8c .. and half + 8c ..
+    const uint32_t d0 = inter ? 16 * c : 8 * c, d1 = inter ? d0 + 8 : half + d0;
+    u4 x0[kHeads], x1[kHeads];
+#pragma unroll
+    for (int n = 0; n < kHeads; ++n) {
+      const uint32_t h = h0 + n;
+      if (h >= h1) continue;
+      const uint16_t* x = h < a.p.NH ? q + h * a.p.D : k + (h - a.p.NH) * a.p.D;
+      x0[n] = *(const u4*)(x + d0);
+      x1[n] = *(const u4*)(x + d1);
+    }
+#pragma unroll
+    for (int n = 0; n < kHeads; ++n) {
+      const uint32_t h = h0 + n;
+      if (h >= h1) continue;
+      u4 y0, y1;
+      if (inter) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float e0 = lo_f(x0[n][w]), o0 = hi_f(x0[n][w]), e1 = lo_f(x1[n][w]), o1 = hi_f(x1[n][w]);
+          y0[w] = pk(e0 * cs[w] - o0 * sn[w], e0 * sn[w] + o0 * cs[w]);
+          y1[w] = pk(e1 * cs[4 + w] - o1 * sn[4 + w], e1 * sn[4 + w] + o1 * cs[4 + w]);
+        }
+      } else {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float a0 = lo_f(x0[n][w]), a1 = hi_f(x0[n][w]), b0 = lo_f(x1[n][w]), b1 = hi_f(x1[n][w]);
+          y0[w] = pk(a0 * cs[2 * w] - b0 * sn[2 * w], a1 * cs[2 * w + 1] - b1 * sn[2 * w + 1]);
+          y1[w] = pk(a0 * sn[2 * w] + b0 * cs[2 * w], a1 * sn[2 * w + 1] + b1 * cs[2 * w + 1]);
+        }
+      }
+      uint16_t* y = h < a.p.NH ? qo + h * a.p.D : ko + (h - a.p.NH) * a.p.D;
+      *(u4*)(y + d0) = y0;
+      *(u4*)(y + d1) = y1;
+    }
+    return;
+  }
+  for (uint32_t h = h0; h < h1; ++h) {
+    const uint16_t* x = h < a.p.NH ? q + h * a.p.D : k + (h - a.p.NH) * a.p.D;
+    uint16_t* y = h < a.p.NH ? qo + h * a.p.D : ko + (h - a.p.NH) * a.p.D;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const uint32_t i = 8 * c + u;
+      if (i >= half) break;
+      const uint32_t e = inter ? 2 * i : i, o = inter ? 2 * i + 1 : half + i;
+      const float xe = __uint_as_float((uint32_t)x[e] << 16), xo = __uint_as_float((uint32_t)x[o] << 16);
+      y[e] = (uint16_t)pk(xe * cs[u] - xo * sn[u], 0.0f);
+      y[o] = (uint16_t)pk(xe * sn[u] + xo * cs[u], 0.0f);
+    }
+  }
+}
+
+bool aligned(const void* p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+bool strides_ok(const metalllmRotaryParams& p, uint64_t heads, uint64_t row, uint64_t seq) {
+  const uint64_t w = heads * p.D;
+  if (row % 8 || seq % 8 || row < w || row >= (1ull << 31) || seq >= (1ull << 48)) return false;
+  if (p.B == 1) return true;
+  return seq >= (p.T - 1) * row + w || (seq >= w && row >= (p.B - 1) * seq + w);
+}
+
+mla::Span span(const metalllmRotaryParams& p, const void* t, uint64_t heads, uint64_t row, uint64_t seq) {
+  return {t, 2 * ((p.B - 1) * seq + (p.T - 1) * row + heads * p.D)};
+}
+
+int rotary(const uint16_t* q, const uint16_t* k, uint16_t* qo, uint16_t* ko, const int32_t* positions,
+           const metalllmRotaryPlan* plan, const metalllmRotaryParams* p, hipStream_t stream, int back) {
+  if (!p || !plan) return METALLLM_ATTN_E_NULL;
+  if (p->D == 0 || p->D % 8 || p->D > 2 * METALLLM_ROTARY_PAIRS) return METALLLM_ATTN_E_HEADDIM;
+  if (p->B == 0 || p->T == 0 || p->NH == 0) return METALLLM_ATTN_E_LAYOUT;
+  if (plan->dims == 0 || plan->dims % 2 || plan->dims > p->D) return METALLLM_ATTN_E_LAYOUT;
+  if (p->B > (1u << 24) || p->T > (1u << 24) || p->NH > (1u << 16) || p->NKV > (1u << 16)) return METALLLM_ATTN_E_SIZE;
+  if (!strides_ok(*p, p->NH, p->q_row, p->q_seq) || !strides_ok(*p, p->NH, p->qo_row, p->qo_seq)) return METALLLM_ATTN_E_LAYOUT;
+  if (p->NKV && (!strides_ok(*p, p->NKV, p->k_row, p->k_seq) || !strides_ok(*p, p->NKV, p->ko_row, p->ko_seq)))
+    return METALLLM_ATTN_E_LAYOUT;
+  if (!q || !qo || (p->NKV && (!k || !ko))) return METALLLM_ATTN_E_NULL;
+  if (!aligned(q, 16) || !aligned(qo, 16) || !aligned(positions, 4)) return METALLLM_ATTN_E_ALIGN;
+  if (p->NKV && (!aligned(k, 16) || !aligned(ko, 16))) return METALLLM_ATTN_E_ALIGN;
+  const uint32_t R = plan->dims, rest = p->D - R;
+  const uint32_t chunks = (R / 2 + 7) / 8 + (rest + 15) / 16, parts = (p->NH + p->NKV + kHeads - 1) / kHeads;
+  const uint64_t work = (uint64_t)p->B * p->T * parts * chunks;
+  if (work >= (1ull << 32) - 256) return METALLLM_ATTN_E_SIZE;
+  const dim3 grid((unsigned)((work + 255) / 256));
+  // A tensor is turned in place (a thread reads and writes the same values) or into memory of its own;
+  // in place, q and k may be interleaved slices of one buffer.
+  const bool q_in = q == qo, k_in = p->NKV && k == ko;
+  if ((q_in && (p->q_row != p->qo_row || p->q_seq != p->qo_seq)) ||
+      (k_in && (p->k_row != p->ko_row || p->k_seq != p->ko_seq)) || (p->NKV && (qo == ko || qo == k || ko == q)))
+    return METALLLM_ATTN_E_OVERLAP;
+  const mla::Span sq = span(*p, q, p->NH, p->q_row, p->q_seq), sqo = span(*p, qo, p->NH, p->qo_row, p->qo_seq);
+  const mla::Span sk = p->NKV ? span(*p, k, p->NKV, p->k_row, p->k_seq) : mla::Span{nullptr, 0};
+  const mla::Span sko = p->NKV ? span(*p, ko, p->NKV, p->ko_row, p->ko_seq) : mla::Span{nullptr, 0};
+  const mla::Span sp{positions, positions ? 4 * (size_t)p->B * p->T : 0};
+  if ((!q_in && mla::any_overlap({sqo}, {sq, sk})) || (p->NKV && !k_in && mla::any_overlap({sko}, {sk, sq})) ||
+      (positions && mla::any_overlap({sp}, {sqo, sko})))
+    return METALLLM_ATTN_E_OVERLAP;
+  const RotArgs a{q, k, qo, ko, positions, *p, *plan};
+  if (R % 16 == 0)
+    hipLaunchKernelGGL(rotary_kernel<true>, grid, dim3(256), 0, stream, a, back, chunks, parts, (uint32_t)work);
+  else
+    hipLaunchKernelGGL(rotary_kernel<false>, grid, dim3(256), 0, stream, a, back, chunks, parts, (uint32_t)work);
+  return hipGetLastError() == hipSuccess ? METALLLM_ATTN_OK : METALLLM_ATTN_E_LAUNCH;
+}
+
+}  // namespace
+
+extern "C" {
+
+int metalllmRotaryPlanInit(uint32_t dims, double base, int interleaved, const metalllmRotaryScaling* sc,
+                           metalllmRotaryPlan* plan) {
+  if (!plan) return METALLLM_ATTN_E_NULL;
+  if (dims == 0 || dims % 2 || dims > 2 * METALLLM_ROTARY_PAIRS || !(base > 0.0) || !std::isfinite(base))
+    return METALLLM_ATTN_E_LAYOUT;
+  const int kind = sc ? sc->kind : METALLLM_ROTARY_PLAIN;
+  if (kind < METALLLM_ROTARY_PLAIN || kind > METALLLM_ROTARY_PARTS) return METALLLM_ATTN_E_LAYOUT;
+  if (kind != METALLLM_ROTARY_PLAIN && (!(sc->factor > 0.0) || !std::isfinite(sc->factor))) return METALLLM_ATTN_E_LAYOUT;
+  if (kind == METALLLM_ROTARY_PARTS && (!(sc->original > 0.0) || !std::isfinite(sc->original) || !std::isfinite(sc->low) ||
+                                        !std::isfinite(sc->high) || !(sc->high > sc->low)))
+    return METALLLM_ATTN_E_LAYOUT;
+  const float magnitude = sc ? sc->magnitude : 1.0f;
+  if (!std::isfinite(magnitude)) return METALLLM_ATTN_E_LAYOUT;
+  metalllmRotaryPlan r{};
+  r.dims = dims, r.interleaved = interleaved != 0, r.magnitude = magnitude;
+  const double two_pi = 6.283185307179586476925286766559;
+  for (uint32_t i = 0; i < dims / 2; ++i) {
+    double f = std::pow(base, -2.0 * i / dims) / two_pi;
+    if (!std::isfinite(f)) return METALLLM_ATTN_E_LAYOUT;
+    if (kind == METALLLM_ROTARY_LINEAR) f /= sc->factor;
+    if (kind == METALLLM_ROTARY_PARTS) {
+      const double keep = std::min(1.0, std::max(0.0, (sc->original * f - sc->low) / (sc->high - sc->low)));
+      f = f * keep + f / sc->factor * (1.0 - keep);
+    }
+    r.turns[i] = f;
+  }
+  *plan = r;
+  return METALLLM_ATTN_OK;
+}
+
+int rotaryForward(const uint16_t* q, const uint16_t* k, uint16_t* q_out, uint16_t* k_out, const int32_t* positions,
+                  const metalllmRotaryPlan* plan, const metalllmRotaryParams* p, metalllm_stream_t stream) {
+  return rotary(q, k, q_out, k_out, positions, plan, p, (hipStream_t)stream, 0);
+}
+
+int rotaryBackward(const uint16_t* dq, const uint16_t* dk, uint16_t* dq_out, uint16_t* dk_out, const int32_t* positions,
+                   const metalllmRotaryPlan* plan, const metalllmRotaryParams* p, metalllm_stream_t stream) {
+  return rotary(dq, dk, dq_out, dk_out, positions, plan, p, (hipStream_t)stream, 1);
+}
+
+}  // extern "C"
