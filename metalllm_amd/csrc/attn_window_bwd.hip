@@ -60,6 +60,12 @@ struct WbCfg {
   static constexpr int DT = D / 32;
 };
 
+// Most tiles of a query block whose rows' Dl is summed over the keys: up to here some row sees 128 keys or
+// fewer. Relative error of dQ, rounded O / summed: T = 44, D = 128 2.8e-3 / X, ...
+constexpr int kExactTiles = 4;
+
+__device__ __forceinline__ void pin(u32x4& a) { asm volatile("" : "+v"(a)); }
+
 template <int V>
 struct IntTag {
   static constexpr int value = V;
@@ -92,7 +98,8 @@ __global__ void __launch_bounds__(256, 2) win_dq_kernel(WinBwdArgs a) {
   uint16_t* dQg = a.dQ + b * s.q_seq + (size_t)ic * s.q_row + head * D;
   const size_t stat = ((size_t)b * s.NH + head) * s.TQ + ic, stats = (size_t)s.B * s.NH * s.TQ;
 
-  // Q^T and dO^T as B operands: lane holds the row, d = 16c + 8h .. +7
+  // Q^T and dO^T as B operands: lane holds the row, d = 16c + 8h .. +7. Dl from dO and the rounded O: half a
+  // step of O's values, which for rows of many keys are small against dP.
   u32x4 Qr[C::KC], Gr[C::KC];
   const uint16_t* Qg = a.q + b * s.q_seq + (size_t)ic * s.q_row + head * D + 8 * h;
   const size_t o_at = b * s.o_seq + (size_t)ic * s.o_row + head * D + 8 * h;
@@ -105,10 +112,6 @@ __global__ void __launch_bounds__(256, 2) win_dq_kernel(WinBwdArgs a) {
   }
   dl = sum_halves(dl);
   const float l2 = a.l[stat] * kLog2e;
-  if (row_ok && h == 0) {
-    a.Dsum[stat] = dl;
-    a.Dsum[stats + stat] = l2;
-  }
   const float sl = s.scale * kLog2e;
 
   const char* Kg = (const char*)(a.k + b * s.k_seq + kvh * D);
@@ -261,25 +264,64 @@ __global__ void __launch_bounds__(256, 2) win_dq_kernel(WinBwdArgs a) {
     }
   };
 
+  // How the wave's rows see the tile of step j: not at all (0), in part (1), or every row every key (2)
+  const int pw0 = sq.off + i0 + 32 * wave, pw1 = min(pw0 + 31, sq.off + i1);
+  auto sight = [&](int j) {
+    const int ka = wt.tile(j) * kTile;
+    if (i0 + 32 * wave > i1 || ka > pw1 || (ka + kTile - 1 <= pw0 - s.window && (ka > 0 || s.sinks == 0))) return 0;
+    return ka + kTile - 1 <= pw0 && pw1 - ka < s.window ? 2 : 1;
+  };
+
+  // Rows of few keys: there the rounding of O is of the size of dP itself, so Dl = sum_j P_ij dP_ij, in a pass
+  // over the tiles of its own (two of the three products again).
+  if (wt.n <= kExactTiles) {
+    dl = 0.0f;
+    for (int j = 0; j < wt.n; ++j) {
+      issue_tile(j);
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();
+      const uint32_t kb = smem_a + (j & 1) * 2 * C::TBYTES + row_rd;
+      const int key0 = wt.tile(j) * kTile + 4 * h;
+#pragma unroll 1
+      for (int t = 0; t < 2 && sight(j); ++t) {
+        f32x16 x = zero16(), y = zero16();
+#pragma unroll
+        for (int c = 0; c < C::KC; ++c) {
+          x = mfma(lds_b128_w(kb + 2 * (32 * t * C::P + 16 * c)), Qr[c], x);
+          y = mfma(lds_b128_w(kb + C::TBYTES + 2 * (32 * t * C::P + 16 * c)), Gr[c], y);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (win_sees(s, pos, key0 + 32 * t + 8 * (r >> 2) + (r & 3))) dl = fmaf(exp2_hw(fmaf(x[r], sl, -l2)), y[r], dl);
+      }
+      __syncthreads();
+    }
+    dl = sum_halves(dl);
+  }
+  if (row_ok && h == 0) {
+    a.Dsum[stat] = dl;
+    a.Dsum[stats + stat] = l2;
+  }
+
   if (wt.n) {
     issue_tile(0);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    const int last = sq.off + i0 + BM - 1, j_of = wt.sink - wt.t0;
-    int f0 = max(1, (max(0, last - s.window + 1) + kTile - 1) / kTile + j_of);
-    int f1 = min(max(0, sq.off + i0 + 1) / kTile + j_of, wt.n);
-    if (f0 >= f1) f0 = f1 = wt.n;
-    auto run = [&](int j, auto tag) __attribute__((always_inline)) {
+    int j = 0;
+    auto run = [&](auto tag) __attribute__((always_inline)) {
       if (j + 1 < wt.n) issue_tile(j + 1);
-      tile(j, tag);
+      if constexpr (decltype(tag)::value >= 0) tile(j, tag);
       __builtin_amdgcn_s_waitcnt(0);
       __syncthreads();
+      ++j;
     };
-    run(0, IntTag<2>());
-    int j = 1;
-    for (; j < f0; ++j) run(j, IntTag<1>());
-    for (; j < f1; ++j) run(j, IntTag<0>());
-    for (; j < wt.n; ++j) run(j, IntTag<1>());
+    if (sight(0) && s.sinks > 0)
+      run(IntTag<2>());
+    while (j < wt.n) {
+      while (j < wt.n && sight(j) == 0) run(IntTag<-1>());
+      while (j < wt.n && sight(j) == 1) run(IntTag<1>());
+      while (j < wt.n && sight(j) == 2) run(IntTag<0>());
+    }
   }
 
   // a hidden key whose row is not finite has added 0 * NaN to the rows of its tile: such rows are summed
@@ -303,6 +345,8 @@ __global__ void __launch_bounds__(256, 2) win_dq_kernel(WinBwdArgs a) {
         float x = 0.0f, y = 0.0f;
 #pragma unroll
         for (int c = 0; c < C::KC; ++c) {
+          pin(Qr[c]);  // (or the unpacked values are kept over the loop)
+          pin(Gr[c]);
           x = dot8(*(const u32x4*)(kr + 16 * c + 8 * h), Qr[c], x);
           y = dot8(*(const u32x4*)(vr + 16 * c + 8 * h), Gr[c], y);
         }
@@ -410,12 +454,13 @@ struct WinKeyWave {
     auto seen = [&](int t, int r) { return (uint32_t)(d0 + 32 * t + 8 * (r >> 2) + (r & 3)) < lim; };
     auto p_pair = [&](f32x16& x, int t, int u, float l0, float l1) {
       const int r = 2 * u;
-      float p0 = exp2_hw(fmaf(x[r], sl, -l0));
-      float p1 = exp2_hw(fmaf(x[r + 1], sl, -l1));
-      if (MASK) {
-        p0 = seen(t, r) ? p0 : 0.0f;
-        p1 = seen(t, r + 1) ? p1 : 0.0f;
+      float p0 = x[r], p1 = x[r + 1];
+      if (MASK) {  // p = 0
+        p0 = seen(t, r) ? p0 : -INFINITY;
+        p1 = seen(t, r + 1) ? p1 : -INFINITY;
       }
+      p0 = exp2_hw(fmaf(p0, sl, -l0));
+      p1 = exp2_hw(fmaf(p1, sl, -l1));
       pin(p0, p1);
       x[r] = p0;
       x[r + 1] = p1;
@@ -425,12 +470,7 @@ struct WinKeyWave {
     };
     auto ds_pair = [&](const f32x16& x, const f32x16& y, int t, int u, float l0, float l1) {
       const int r = 2 * u;
-      float e0 = x[r] * (y[r] - l0), e1 = x[r + 1] * (y[r + 1] - l1);
-      if (MASK) {  // a hidden row's dP or Dl may not be finite
-        e0 = seen(t, r) ? e0 : 0.0f;
-        e1 = seen(t, r + 1) ? e1 : 0.0f;
-      }
-      uint32_t pk = pack_bf16(e0, e1);
+      uint32_t pk = pack_bf16(x[r] * (y[r] - l0), x[r + 1] * (y[r + 1] - l1));
       pin(pk);
       dS[8 * t + u] = pk;
     };
@@ -569,35 +609,40 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) win_dkdv_kernel(WinBwdAr
       dma4_v(p, dst + C::STAT + 256);
     }
   };
-  // tiles that every key of the block is seen from (far: the sink keys), without a row past the end
-  auto whole = [&](int t) {
-    const int p0 = sq.off + t * kTile;
-    return t * kTile + kTile <= sq.lq && (far || (p0 >= k0 + BN - 1 && p0 + kTile - 1 - k0 < s.window));
+  // How tile t sees the wave's 32 keys: not at all (0), in part (1), or every row every key (2; far: the sinks)
+  const int kw0 = k0 + 32 * wave, kw1 = min(kw0 + 31, k1);
+  auto sight = [&](int t) {
+    const int p0 = sq.off + t * kTile, p1 = p0 + kTile - 1;
+    const bool sink = kw0 < s.sinks;
+    if (kw0 > k1 || (far && !sink) || p1 < kw0 || (p0 - kw1 >= s.window && !sink)) return 0;
+    return t * kTile + kTile <= sq.lq && (far || (p0 >= kw1 && p1 - kw0 < s.window)) ? 2 : 1;
   };
 
   if (f0 < f1) {
-    int g = f0 / nt, t = tlo + f0 - g * nt;
+    int f = f0, g = f0 / nt, t = tlo + f0 - g * nt;  // item f: query tile t of head g
     issue_tile(g, t, 0);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    for (int f = f0; f < f1; ++f) {
+    // the next item is copied while `step` runs on this one
+    auto item = [&](auto step) __attribute__((always_inline)) {
       int gn = g, tn = t + 1;
       if (tn == tlo + nt) {
         tn = tlo;
         ++gn;
       }
       if (f + 1 < f1) issue_tile(gn, tn, (f + 1 - f0) & 1);
-      const uint32_t st_a = smem_a + ((f - f0) & 1) * C::STAGE;
-      if (wave_on) {
-        if (whole(t))
-          wv.template step<false>(st_a, 0, 0);
-        else
-          wv.template step<true>(st_a, sq.off + t * kTile + 4 * h - key, lim);
-      }
+      step(smem_a + ((f - f0) & 1) * C::STAGE);
       __builtin_amdgcn_s_waitcnt(0);
       __syncthreads();
-      g = gn;
-      t = tn;
+      ++f, g = gn, t = tn;
+    };
+    // loops of one form of the step each (a choice inside one loop costs a copy of the sums per tile); every
+    // wave passes every item's barrier
+    while (f < f1) {
+      while (f < f1 && sight(t) == 0) item([](uint32_t) {});
+      while (f < f1 && sight(t) == 1)
+        item([&](uint32_t st) { wv.template step<true>(st, sq.off + t * kTile + 4 * h - key, lim); });
+      while (f < f1 && sight(t) == 2) item([&](uint32_t st) { wv.template step<false>(st, 0, 0); });
     }
   }
 
@@ -624,6 +669,8 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) win_dkdv_kernel(WinBwdAr
           float x = 0.0f, y = 0.0f;
 #pragma unroll
           for (int c = 0; c < C::KC; ++c) {
+            pin(wv.Kr[c]);
+            pin(wv.Vr[c]);
             x = dot8(*(const u32x4*)(qr + 16 * c + 8 * h), wv.Kr[c], x);
             y = dot8(*(const u32x4*)(gr + 16 * c + 8 * h), wv.Vr[c], y);
           }

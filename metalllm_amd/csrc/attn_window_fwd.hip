@@ -11,9 +11,9 @@
 // of 64 keys go global -> LDS by direct copies, two stages deep. Step j of the pipeline runs the softmax of
 // tile j on the vector ALU between the matrix products of S of tile j + 1 and P.V of tile j - 1.
 //
-// Masks: only tiles that some row of the workgroup sees in part run the masked step, one unsigned compare
-// per score: (uint)(pos - key) < window is both the causal border and the window's. The sinks add a
-// compare in the first step alone, since they all lie in tile 0, which comes first.
+// Masks: a wave skips the tiles that none of its rows sees, and masks those that its rows see in part, before
+// the step: one unsigned compare per score, since (uint)(pos - key) < window is both the causal border and
+// the window's. The sinks add a compare in tile 0, which holds all of them and comes first.
 //
 // The reference point m moves only when a tile's max exceeds it by 2^8 in the exponent's base (l and O
 // are fp32 and p keeps its relative precision under any reference point), so O is rarely rescaled.
@@ -21,7 +21,7 @@
 // Keys that no row of the workgroup sees are never read (their rows are replaced by a visible one and
 // masked). A hidden key whose value row is not finite would still add 0 * NaN to the rows that do not see
 // it but share its tile: rows that end up not finite are summed again one visible key at a time.
-#include <algorithm>
+#include <type_traits>
 
 #include "attn_common.hpp"
 #include "attn_window.hpp"
@@ -44,16 +44,14 @@ struct WfCfg {
   static constexpr int DT = D / 32;
 };
 
-// What a pipeline step does: S of the next tile, P.V of the previous one, the softmax of this one, and
-// its mask (0 none, 1 window and causal border, 2 the sinks too).
-template <bool S_, bool PV_, bool SM_, int MASK_>
+// What a pipeline step does: S of the next tile, P.V of the previous one, the softmax of this one.
+template <bool S_, bool PV_, bool SM_>
 struct WfStep {
   static constexpr bool S = S_, PV = PV_, SM = SM_;
-  static constexpr int MASK = MASK_;
 };
 
 template <int D>
-__global__ void __launch_bounds__(256, 2) win_fwd_kernel(WinFwdArgs a) {
+__global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_fwd_kernel(WinFwdArgs a) {
   using C = WfCfg<D>;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * C::STAGE];
 
@@ -167,9 +165,9 @@ __global__ void __launch_bounds__(256, 2) win_fwd_kernel(WinFwdArgs a) {
   // One step: the products in a fixed order, one per slot (P.V first, then S), each slot with the operand
   // reads of a later one and a slice of the softmax that does not depend on it. Scheduling fences keep the
   // order. Xc = S^T of tile j (in), Xn = S^T of tile j + 1 (out), Pin = P of tile j - 1, Pout = P of tile j.
-  // Softmax: slots [0, BSLOT) mask and max of the score pairs, BSLOT the reference point, then exponent,
+  // Softmax: slots [0, BSLOT) max of the score pairs, BSLOT the reference point, then exponent,
   // exp2, and sum and packed P in three stages per pair.
-  auto wstep = [&](auto flags, int j, int rd, f32x16& Xc0, f32x16& Xc1, f32x16& Xn0, f32x16& Xn1,
+  auto wstep = [&](auto flags, int rd, const f32x16& Xc0, const f32x16& Xc1, f32x16& Xn0, f32x16& Xn1,
                    const uint32_t(&Pin)[16], uint32_t(&Pout)[16]) __attribute__((always_inline)) {
     using F = decltype(flags);
     if (F::PV && rescale) {
@@ -206,14 +204,6 @@ __global__ void __launch_bounds__(256, 2) win_fwd_kernel(WinFwdArgs a) {
       if (n < NM) ring[n] = operand(n);
     float mxa = -INFINITY, mxb = -INFINITY, ls0 = 0.0f, ls1 = 0.0f, mb = 0.0f;
     float t0[16], t1[16], e0[16], e1[16];
-    // key of element e = 64 kt + 4h + off(e): visible where (uint)(dq - off) < window, or off < sq_
-    int dq = 0, sq_ = 0;
-    if (F::MASK) {
-      const int kt = wt.tile(j);
-      dq = pos - kt * C::BN - 4 * h;
-      asm volatile("" : "+v"(dq));
-      if (F::MASK == 2) sq_ = min(s.sinks - kt * C::BN - 4 * h, dq + 1);
-    }
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
       if (n < NM) {
@@ -234,18 +224,8 @@ __global__ void __launch_bounds__(256, 2) win_fwd_kernel(WinFwdArgs a) {
 #pragma unroll
         for (int p = 0; p < 16; ++p)
           if (n == p / APS) {
-            f32x16& Xs = p < 8 ? Xc0 : Xc1;
-            float a0 = Xs[(2 * p) & 15], a1 = Xs[(2 * p + 1) & 15];
-            if (F::MASK) {
-              const int e = 2 * p, off = 32 * (e >> 4) + 8 * ((e & 15) >> 2) + (e & 3);
-              const bool v0 = (uint32_t)(dq - off) < (uint32_t)s.window || (F::MASK == 2 && off < sq_);
-              const bool v1 = (uint32_t)(dq - off - 1) < (uint32_t)s.window || (F::MASK == 2 && off + 1 < sq_);
-              a0 = v0 ? a0 : -INFINITY;
-              a1 = v1 ? a1 : -INFINITY;
-              pin(a0, a1);
-              Xs[(2 * p) & 15] = a0;
-              Xs[(2 * p + 1) & 15] = a1;
-            }
+            const f32x16& Xs = p < 8 ? Xc0 : Xc1;
+            const float a0 = Xs[(2 * p) & 15], a1 = Xs[(2 * p + 1) & 15];
             if (p & 1)
               mxb = max3f(mxb, a0, a1);
             else
@@ -299,61 +279,100 @@ __global__ void __launch_bounds__(256, 2) win_fwd_kernel(WinFwdArgs a) {
     __syncthreads();
   };
   // Step j: every wave copies K(j + 2) and V(j) into stage j & 1, which the steps before have finished
-  // reading, runs the step, then all wait for the copies.
+  // reading, runs its part, then all wait for the copies. Every wave passes every step's barrier.
   const int n = wt.n;
-  auto run = [&](auto flags, int j) __attribute__((always_inline)) {
-    using F = decltype(flags);
+  auto copy = [&](int j) __attribute__((always_inline)) {
     if (j + 2 < n) load_k(j + 2, j & 1);
     load_v(j, j & 1);
-    wstep(flags, j, (j + 1) & 1, Sc0, Sc1, Sn0, Sn1, Pp, Pc);
-    if (F::S) {
-      Sc0 = Sn0;
-      Sc1 = Sn1;
-    }
-#pragma unroll
-    for (int t = 0; t < 16; ++t) Pp[t] = Pc[t];
-    sync();
   };
-
-  load_k(0, 0);
-  if (n > 1) load_k(1, 1);
-  sync();
-  {  // S of the first tile
-    const uint16_t* kb = (const uint16_t*)smem + k_rd;
+  auto scores = [&](int j) __attribute__((always_inline)) {  // S of tile j into Sc
+    const uint16_t* kb = (const uint16_t*)(smem + (j & 1) * C::STAGE) + k_rd;
+    Sc0 = zero16();
+    Sc1 = zero16();
 #pragma unroll
     for (int c = 0; c < C::KC; ++c) {
       Sc0 = mfma(lds_read16(kb + 16 * c), Qr[c], Sc0);
       Sc1 = mfma(lds_read16(kb + 32 * C::KP + 16 * c), Qr[c], Sc1);
     }
-  }
-  __syncthreads();
-  // steps [f0, f1) of the tiles that every row of the workgroup sees whole
-  const int last = sq.off + i0 + C::BM - 1;
+  };
+  // This wave's rows [pw0, pw1] (positions) see tiles of the steps jw0 .. jw1 (and, behind the sink tile,
+  // up to two that only its neighbours see: masked whole).
+  const int pw0 = sq.off + i0 + 32 * wave, pw1 = min(pw0 + 31, sq.off + i1);
   const int j_of = wt.sink - wt.t0;  // step of window tile kt: kt + j_of
-  int f0 = max(1, (max(0, last - s.window + 1) + C::BN - 1) / C::BN + j_of);
-  int f1 = (max(0, sq.off + i0 + 1)) / C::BN + j_of;
-  f1 = min(f1, n - 1);
-  if (f0 >= f1) f0 = f1 = n - 1;
-  if (n == 1)
-    run(WfStep<false, false, true, 2>(), 0);
-  else
-    run(WfStep<true, false, true, 2>(), 0);
-  int j = 1;
-  for (; j < f0; ++j) run(WfStep<true, true, true, 1>(), j);
-  if (j < f1 && ((f1 - j) & 1)) run(WfStep<true, true, true, 0>(), j++);
-  for (; j + 1 < f1; j += 2) {  // two steps in turn on swapped buffers
-    if (j + 2 < n) load_k(j + 2, j & 1);
-    load_v(j, j & 1);
-    wstep(WfStep<true, true, true, 0>(), j, (j + 1) & 1, Sc0, Sc1, Sn0, Sn1, Pp, Pc);
+  const bool active = i0 + 32 * wave <= i1 && pw1 >= 0;
+  const int jw0 = !active ? n + 1 : s.sinks > 0 ? 0 : max(0, pw0 - s.window + 1) / C::BN + j_of;
+  const int jw1 = active ? pw1 / C::BN + j_of : -1;
+  auto mask = [&](auto first, int j, f32x16& X0, f32x16& X1) __attribute__((always_inline)) {
+    const int ka = wt.tile(j) * C::BN;
+    if (ka + C::BN - 1 <= pw0 && pw0 + 31 - ka < s.window) return;  // seen whole
+    int dq = pos - ka - 4 * h;  // score r of half t is key ka + 4h + off
+    asm volatile("" : "+v"(dq));  // (opaque: 32 loop-invariant bounds would be kept instead)
+    // keys ka + 4h + off < sinks: the sinks are in tile 0, and that is the wave's first one then
+    const int few = decltype(first)::value ? min(s.sinks - ka - 4 * h, dq + 1) : 0;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+      const int off = 32 * (e >> 4) + 8 * ((e & 15) >> 2) + (e & 3);
+      f32x16& X = e < 16 ? X0 : X1;
+      const bool seen = (uint32_t)(dq - off) < (uint32_t)s.window || (decltype(first)::value && off < few);
+      X[e & 15] = seen ? X[e & 15] : -INFINITY;
+    }
+  };
+  int j = 0;
+  auto run = [&](auto flags) __attribute__((always_inline)) {
+    using F = decltype(flags);
+    if (j < n) copy(j);
+    if (F::SM) mask(std::bool_constant<!F::PV>(), j, Sc0, Sc1);
+    wstep(flags, (j + 1) & 1, Sc0, Sc1, Sn0, Sn1, Pp, Pc);
+    if (F::S) {
+      Sc0 = Sn0;
+      Sc1 = Sn1;
+    }
+    if (F::SM) {
+#pragma unroll
+      for (int t = 0; t < 16; ++t) Pp[t] = Pc[t];
+    }
+    if (j < n) sync();
+    ++j;
+  };
+
+  load_k(0, 0);
+  if (n > 1) load_k(1, 1);
+  sync();
+  if (jw0 == 0) scores(0);
+  __syncthreads();
+  while (j < min(jw0 - 1, n)) {
+    copy(j);
     sync();
-    if (j + 3 < n) load_k(j + 3, (j + 1) & 1);
-    load_v(j + 1, (j + 1) & 1);
-    wstep(WfStep<true, true, true, 0>(), j + 1, j & 1, Sn0, Sn1, Sc0, Sc1, Pc, Pp);
-    sync();
+    ++j;
   }
-  for (; j < n - 1; ++j) run(WfStep<true, true, true, 1>(), j);
-  if (j < n) run(WfStep<false, true, true, 1>(), j);
-  wstep(WfStep<false, true, false, 0>(), n, (n - 1) & 1, Sc0, Sc1, Sn0, Sn1, Pp, Pc);
+  if (active) {
+    if (jw0 > 0) {  // step jw0 - 1
+      copy(j);
+      scores(jw0);
+      sync();
+      ++j;
+    }
+    run(WfStep<true, false, true>());  // (behind the wave's last tile S is of no use, and unused)
+    if (j < jw1 && ((jw1 - j) & 1)) run(WfStep<true, true, true>());
+    while (j < jw1) {  // two steps in turn on swapped buffers
+      copy(j);
+      mask(std::false_type(), j, Sc0, Sc1);
+      wstep(WfStep<true, true, true>(), (j + 1) & 1, Sc0, Sc1, Sn0, Sn1, Pp, Pc);
+      sync();
+      copy(j + 1);
+      mask(std::false_type(), j + 1, Sn0, Sn1);
+      wstep(WfStep<true, true, true>(), j & 1, Sn0, Sn1, Sc0, Sc1, Pc, Pp);
+      sync();
+      j += 2;
+    }
+    if (j == jw1) run(WfStep<false, true, true>());
+    run(WfStep<false, true, false>());
+  }
+  while (j < n) {
+    copy(j);
+    sync();
+    ++j;
+  }
 
   // ---- out = bf16(O / l), l = m/sqrt(D) + ln(sum) ----
   const float lt = sum_halves(l_run);
@@ -378,6 +397,7 @@ __global__ void __launch_bounds__(256, 2) win_fwd_kernel(WinFwdArgs a) {
         float x = 0.0f;
 #pragma unroll
         for (int c = 0; c < C::KC; ++c) {
+          asm volatile("" : "+v"(Qr[c]));  // (or the unpacked values are kept over the loop)
           const u32x4 kk = *(const u32x4*)(kr + 16 * c + 8 * h);
 #pragma unroll
           for (int w = 0; w < 4; ++w) {

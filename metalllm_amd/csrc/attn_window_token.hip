@@ -11,7 +11,8 @@
 //     agree, so p needs no exchange.
 //   * V rows are loaded whole (16 lanes x 16 or 8 bytes), the lane's 8 keys of its d chunk, and turned in
 //     registers: one v_perm per pair of values. The d of an output row is E*(4g + r) + e for product e.
-// A step takes 32 keys; the next step's 64 registers of K and V are loaded while one is computed.
+// A step takes 32 keys. Its K registers are loaded again as soon as its scores are formed, its V registers
+// as soon as its products are; the loads of three waves per SIMD cover the rest.
 //
 // Split: the steps are dealt to the 4 waves of a workgroup, and over `splits` workgroups where there are
 // too few (sequence, key head) pairs to fill the chip; each part keeps its own reference point and sum, and
@@ -72,14 +73,10 @@ __device__ __forceinline__ WtRange wt_range(const WinShape& s, const WinSeq& q, 
   return r;
 }
 
-template <int D>
-struct WtStep {
-  u32x4 k[2][WtCfg<D>::KC];
-  uint32_t v[8][WtCfg<D>::VW];
-};
-
-template <int D>
-__global__ void __launch_bounds__(256, 2) win_token_kernel(WinFwdArgs a) {
+// SEVERAL: more than one query row (TQ > 1), which may see different keys of a step; its path for values that
+// are not finite takes registers that one row does without.
+template <int D, bool SEVERAL>
+__global__ void __launch_bounds__(256, SEVERAL ? 2 : D == 64 ? 4 : 3) win_token_kernel(WinFwdArgs a) {
   using C = WtCfg<D>;
   __shared__ __attribute__((aligned(16))) float sm_o[4][kTokRows][C::PITCH];
   __shared__ float sm_m[4][kTokRows], sm_l[4][kTokRows];
@@ -112,7 +109,6 @@ __global__ void __launch_bounds__(256, 2) win_token_kernel(WinFwdArgs a) {
   const char* Vg = (const char*)(a.v + b * s.v_seq + kvh * D);
   const uint32_t krs = 2 * s.k_row, vrs = 2 * s.v_row;
   const float c1 = s.scale * kLog2e, slack = 8.0f / c1;
-  const bool several = w.i_lo != w.i_hi;  // rows that may see different keys
 
   // first key of step t and one past its last
   auto keys_of = [&](int t, int& base, int& end) {
@@ -122,29 +118,34 @@ __global__ void __launch_bounds__(256, 2) win_token_kernel(WinFwdArgs a) {
   };
   // V row x of the lane: key 4g + x, or 16 + 4g + x - 4
   auto v_key = [&](int x) { return 4 * g + x + (x >= 4 ? 12 : 0); };
-  auto load = [&](int t, WtStep<D>& st) __attribute__((always_inline)) {
+  u32x4 kk[2][C::KC];      // the lane's two K rows of a step
+  uint32_t vv[8][C::VW];  // its 8 V rows
+  auto load_k = [&](int t) __attribute__((always_inline)) {
     int base, end;
     keys_of(t, base, end);
-    const int most = end - 1 - base;
     const char* kp = Kg + (size_t)base * krs;
-    const char* vp = Vg + (size_t)base * vrs;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const char* p = kp + __umul24(min(16 * u + n16, most), krs) + 16 * g;
+      const uint32_t at = __umul24(min(16 * u + n16, end - 1 - base), krs) + 16 * g;
 #pragma unroll
-      for (int c = 0; c < C::KC; ++c) st.k[u][c] = *(const u32x4*)(p + 64 * c);
+      for (int c = 0; c < C::KC; ++c) kk[u][c] = *(const u32x4*)(kp + at + 64 * c);
     }
+  };
+  auto load_v = [&](int t) __attribute__((always_inline)) {
+    int base, end;
+    keys_of(t, base, end);
+    const char* vp = Vg + (size_t)base * vrs;
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
-      const char* p = vp + __umul24(min(v_key(x), most), vrs) + 4 * C::VW * n16;
+      const uint32_t at = __umul24(min(v_key(x), end - 1 - base), vrs) + 4 * C::VW * n16;
       if constexpr (C::VW == 4) {
-        const u32x4 y = *(const u32x4*)p;
+        const u32x4 y = *(const u32x4*)(vp + at);
 #pragma unroll
-        for (int d = 0; d < 4; ++d) st.v[x][d] = y[d];
+        for (int d = 0; d < 4; ++d) vv[x][d] = y[d];
       } else {
-        const u32x2v y = *(const u32x2v*)p;
-        st.v[x][0] = y[0];
-        st.v[x][1] = y[1];
+        const u32x2v y = *(const u32x2v*)(vp + at);
+        vv[x][0] = y[0];
+        vv[x][1] = y[1];
       }
     }
   };
@@ -155,22 +156,23 @@ __global__ void __launch_bounds__(256, 2) win_token_kernel(WinFwdArgs a) {
   float m_run = -INFINITY, l_run = 0.0f;
 
   // V^T operand of product e: d = E*lane%16 + e, the lane's 8 keys
-  auto turned = [&](const uint32_t(&v)[8][C::VW], int e) {
+  auto turned = [&](int e) {
     u32x4 r;
 #pragma unroll
     for (int d = 0; d < 4; ++d)
-      r[d] = __builtin_amdgcn_perm(v[2 * d + 1][e / 2], v[2 * d][e / 2], (e & 1) ? 0x07060302u : 0x05040100u);
+      r[d] = __builtin_amdgcn_perm(vv[2 * d + 1][e / 2], vv[2 * d][e / 2], (e & 1) ? 0x07060302u : 0x05040100u);
     return r;
   };
-  auto compute = [&](int t, const WtStep<D>& st) __attribute__((always_inline)) {
+  auto step = [&](int t) __attribute__((always_inline)) {
     int base, end;
     keys_of(t, base, end);
     f32x4 S[2] = {f32x4{0, 0, 0, 0}, f32x4{0, 0, 0, 0}};
 #pragma unroll
     for (int c = 0; c < C::KC; ++c) {
-      S[0] = mfma16(st.k[0][c], Qr[c], S[0]);
-      S[1] = mfma16(st.k[1][c], Qr[c], S[1]);
+      S[0] = mfma16(kk[0][c], Qr[c], S[0]);
+      S[1] = mfma16(kk[1][c], Qr[c], S[1]);
     }
+    if (t + 1 < t1) load_k(t + 1);
     float mt = -INFINITY;
 #pragma unroll
     for (int u = 0; u < 2; ++u)
@@ -199,43 +201,42 @@ __global__ void __launch_bounds__(256, 2) win_token_kernel(WinFwdArgs a) {
     }
     const u32x4 P = {pack_bf16(p[0], p[1]), pack_bf16(p[2], p[3]), pack_bf16(p[4], p[5]), pack_bf16(p[6], p[7])};
     bool odd = false;
-    if (several) {
+    if (SEVERAL) {
 #pragma unroll
       for (int x = 0; x < 8; ++x)
 #pragma unroll
-        for (int d = 0; d < C::VW; ++d) odd |= not_finite(st.v[x][d]);
+        for (int d = 0; d < C::VW; ++d) odd |= not_finite(vv[x][d]);
     }
-    if (!__any(odd)) {
+    if (!SEVERAL || !__any(odd)) {
 #pragma unroll
-      for (int e = 0; e < C::E; ++e) O[e] = mfma16(turned(st.v, e), P, O[e]);
+      for (int e = 0; e < C::E; ++e) O[e] = mfma16(turned(e), P, O[e]);
     } else {  // values that are not finite: query row by query row, without the keys that it does not see
       for (int i = w.i_lo; i <= w.i_hi; ++i) {
-        uint32_t v[8][C::VW];
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const int key = base + v_key(x);
-          const bool sees = key < end && win_sees(s, sq.off + i, key);
+        for (int x = 0; x < 8; ++x)
 #pragma unroll
-          for (int d = 0; d < C::VW; ++d) v[x][d] = sees ? st.v[x][d] : 0u;
+          for (int d = 0; d < C::VW; ++d) pin(vv[x][d]);  // (or the turned operands are kept over the loop)
+        u32x4 kept;  // of the pairs of keys in an operand
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const int k0 = base + v_key(2 * d), k1 = base + v_key(2 * d + 1);
+          kept[d] = (k0 < end && win_sees(s, sq.off + i, k0) ? 0xffffu : 0u) |
+                    (k1 < end && win_sees(s, sq.off + i, k1) ? 0xffff0000u : 0u);
         }
 #pragma unroll
         for (int e = 0; e < C::E; ++e) {
-          const f32x4 y = mfma16(turned(v, e), P, O[e]);
+          const f32x4 y = mfma16(turned(e) & kept, P, O[e]);
           if (qi == i) O[e] = y;
         }
       }
     }
+    if (t + 1 < t1) load_v(t + 1);
   };
 
   if (t0 < t1) {
-    WtStep<D> s0, s1;
-    load(t0, s0);
-    for (int t = t0; t < t1; t += 2) {
-      if (t + 1 < t1) load(t + 1, s1);
-      compute(t, s0);
-      if (t + 2 < t1) load(t + 2, s0);
-      if (t + 1 < t1) compute(t + 1, s1);
-    }
+    load_k(t0);
+    load_v(t0);
+    for (int t = t0; t < t1; ++t) step(t);
   }
 
   // ---- join the waves ----
@@ -325,21 +326,21 @@ __global__ void __launch_bounds__(256) win_join_kernel(WinFwdArgs a) {
     a.l[((size_t)b * s.NH + head) * s.TQ + qi] = empty ? -INFINITY : M * (1.0f / kLog2e) + logf(L);
 }
 
-// Workgroups per (sequence, key head, row tile): enough for two per CU, each wave keeping two steps or more.
+// Workgroups per (sequence, key head, row tile): enough for three per CU, each wave keeping two steps or more.
 int win_token_splits(const WinShape& s) {
   const int64_t units = (int64_t)s.B * s.NKV * (((int64_t)s.TQ * s.G + kTokRows - 1) / kTokRows);
   const int64_t keys = std::min<int64_t>((int64_t)s.window + s.TQ - 1, s.TK) + s.sinks;
   const int64_t steps = (keys + 31) / 32;
-  const int64_t want = std::min<int64_t>((2 * kCus + units - 1) / units, steps / 8);
+  const int64_t want = std::min<int64_t>((3 * kCus + units - 1) / units, steps / 8);
   return (int)std::max<int64_t>(1, std::min<int64_t>(want, 64));
 }
 
 hipError_t launch_window_token(const WinFwdArgs& a, int D, hipStream_t s) {
   const unsigned units = (unsigned)(a.s.B * a.s.NKV * ((a.s.TQ * a.s.G + kTokRows - 1) / kTokRows));
-  if (D == 64)
-    hipLaunchKernelGGL(win_token_kernel<64>, dim3(units * a.splits), dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL(win_token_kernel<128>, dim3(units * a.splits), dim3(256), 0, s, a);
+  const bool several = a.s.TQ > 1;
+  auto kernel = D == 64 ? (several ? win_token_kernel<64, true> : win_token_kernel<64, false>)
+                        : (several ? win_token_kernel<128, true> : win_token_kernel<128, false>);
+  hipLaunchKernelGGL(kernel, dim3(units * a.splits), dim3(256), 0, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
   if (D == 64)

@@ -54,21 +54,22 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotArgs a, int back, uint32
   uint16_t* qo = a.qo + b * a.p.qo_seq + t * a.p.qo_row;
   uint16_t* ko = a.ko + b * a.p.ko_seq + t * a.p.ko_row;
 
-  if (c >= turning) {  // the part of the head behind the first R: values R + 16 (c - turning) ..
-    const uint32_t d0 = R + 16 * (c - turning), d1 = min(d0 + 16, a.p.D);
-    for (uint32_t h = h0; h < h1; ++h) {
-      const bool isq = h < a.p.NH;
-      const uint16_t* x = isq ? q + h * a.p.D : k + (h - a.p.NH) * a.p.D;
-      uint16_t* y = isq ? qo + h * a.p.D : ko + (h - a.p.NH) * a.p.D;
-      if (x == y) continue;
-      if (VEC) {  // R, hence d0, is a multiple of 16, D of 8
-        *(u4*)(y + d0) = *(const u4*)(x + d0);
-        if (d0 + 8 < d1) *(u4*)(y + d0 + 8) = *(const u4*)(x + d0 + 8);
-      } else {
-        for (uint32_t d = d0; d < d1; ++d) y[d] = x[d];
-      }
+  const bool copied = c >= turning;  // the part of the head behind the first R: values R + 16 (c - turning) ..
+  const bool inter = a.plan.interleaved != 0;
+  // VEC: the thread's two 16-byte chunks of a head: values 16c .. 16c + 15 (neighbours paired, or copied) or
+  // 8c .. and half + 8c ..; every load is in flight while the sines are computed
+  const uint32_t d0 = copied ? R + 16 * (c - turning) : inter ? 16 * c : 8 * c;
+  const uint32_t d1 = copied || inter ? d0 + 8 : half + d0;
+  const bool two = d1 < a.p.D;
+  u4 x0[kHeads], x1[kHeads];
+  if (VEC) {
+#pragma unroll
+    for (int n = 0; n < kHeads; ++n) {
+      const uint32_t h = min(h0 + n, h1 - 1);
+      const uint16_t* x = h < a.p.NH ? q + h * a.p.D : k + (h - a.p.NH) * a.p.D;
+      x0[n] = *(const u4*)(x + d0);
+      x1[n] = two ? *(const u4*)(x + d1) : u4{0, 0, 0, 0};
     }
-    return;
   }
   const double pos = a.pos ? (double)a.pos[token] : (double)t;
   float cs[8], sn[8];
@@ -82,19 +83,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotArgs a, int back, uint32
     sn[u] = __builtin_amdgcn_sinf(f) * a.plan.magnitude;
     if (back) sn[u] = -sn[u];
   }
-  const bool inter = a.plan.interleaved != 0;
   if (VEC) {
-    // two 16-byte chunks of a head: values 16c .. 16c + 15 (neighbours paired) or 8c .. and half + 8c ..
-    const uint32_t d0 = inter ? 16 * c : 8 * c, d1 = inter ? d0 + 8 : half + d0;
-    u4 x0[kHeads], x1[kHeads];
-#pragma unroll
-    for (int n = 0; n < kHeads; ++n) {
-      const uint32_t h = h0 + n;
-      if (h >= h1) continue;
-      const uint16_t* x = h < a.p.NH ? q + h * a.p.D : k + (h - a.p.NH) * a.p.D;
-      x0[n] = *(const u4*)(x + d0);
-      x1[n] = *(const u4*)(x + d1);
-    }
 #pragma unroll
     for (int n = 0; n < kHeads; ++n) {
       const uint32_t h = h0 + n;
@@ -116,8 +105,17 @@ __global__ void __launch_bounds__(256) rotary_kernel(RotArgs a, int back, uint32
         }
       }
       uint16_t* y = h < a.p.NH ? qo + h * a.p.D : ko + (h - a.p.NH) * a.p.D;
-      *(u4*)(y + d0) = y0;
-      *(u4*)(y + d1) = y1;
+      *(u4*)(y + d0) = copied ? x0[n] : y0;
+      if (two) *(u4*)(y + d1) = copied ? x1[n] : y1;
+    }
+    return;
+  }
+  if (copied) {
+    for (uint32_t h = h0; h < h1; ++h) {
+      const uint16_t* x = h < a.p.NH ? q + h * a.p.D : k + (h - a.p.NH) * a.p.D;
+      uint16_t* y = h < a.p.NH ? qo + h * a.p.D : ko + (h - a.p.NH) * a.p.D;
+      if (x == y) continue;
+      for (uint32_t d = d0; d < min(d0 + 16, a.p.D); ++d) y[d] = x[d];
     }
     return;
   }
