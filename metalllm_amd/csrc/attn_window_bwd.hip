@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(256, 2) win_dq_kernel(WinBwdArgs a) {
     f32x16 x0 = zero16(), x1 = zero16(), y0 = zero16(), y1 = zero16();
     uint32_t dS[16];
     constexpr int RING = 6;
-    auto ahead = [](int n) { return n < 2 * C::KC ? 5 : 2; };
+    auto ahead = [](int n) { return n < 2 * C::KC || D == 64 ? 5 : 4; };
     u32x4 ring[RING];
     auto op_of = [&](int n) -> u32x4 {
       if (n < 4 * C::KC) {
@@ -474,9 +474,9 @@ struct WinKeyWave {
       pin(pk);
       dS[8 * t + u] = pk;
     };
-    constexpr int RING = 5;
-    constexpr int SA = 2;
-    auto ahead = [](int i) { return i < C::KC ? 4 : 2; };
+    constexpr int RING = D == 64 ? 5 : 7;
+    constexpr int SA = 3;
+    auto ahead = [](int) { return RING - 1; };
     u32x4 ring[RING];
     f32x4 sring[SA + 1];
 #pragma unroll

@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_fwd_kernel(WinFwdArg
       const int t = n - NPV;
       return lds_read16(kb + (t & 1) * 32 * C::KP + 16 * (t >> 1));
     };
-    constexpr int RING = 4;
+    constexpr int RING = D == 64 ? 4 : 6;
     u32x4 ring[RING];
 #pragma unroll
     for (int n = 0; n < RING - 1; ++n)
