@@ -58,6 +58,12 @@ struct WbCfg {
   static constexpr int STAGE = 2 * TBYTES + 512;
   static constexpr int KC = D / 16;
   static constexpr int DT = D / 32;
+  // Byte offset, from a tile's first row, of what the lane copies in the wave's instruction n: 16-byte slot t
+  // of the padded tile, row t / SLOTS held in [lo, hi], pad chunks repeating the row's last one.
+  __device__ static __forceinline__ uint32_t copy_offset(int wave, int lane, int n, int lo, int hi, uint32_t row_bytes) {
+    const int t = 64 * (wave + 4 * n) + lane, r = t / SLOTS;
+    return __umul24(clamp_row(r, lo, hi), row_bytes) + 16 * min(t - r * SLOTS, D / 8 - 1);
+  }
 };
 
 // Most tiles of a query block whose rows' Dl is summed over the keys: up to here some row sees 128 keys or
@@ -117,14 +123,10 @@ __global__ void __launch_bounds__(256, 2) win_dq_kernel(WinBwdArgs a) {
   const char* Kg = (const char*)(a.k + b * s.k_seq + kvh * D);
   const char* Vg = (const char*)(a.v + b * s.v_seq + kvh * D);
   const uint32_t krs = 2 * s.k_row, vrs = 2 * s.v_row;
-  int crow[C::LPW];
-  uint32_t cchunk[C::LPW];
+  // bytes of the copies' rows from the tile's first (attn_window_fwd.hip)
+  uint32_t koff[C::LPW];  // k's, and v's where its rows are as far apart
 #pragma unroll
-  for (int j = 0; j < C::LPW; ++j) {
-    const int t = 64 * (wave + 4 * j) + lane;
-    crow[j] = t / C::SLOTS;
-    cchunk[j] = 16 * min(t % C::SLOTS, D / 8 - 1);
-  }
+  for (int n = 0; n < C::LPW; ++n) koff[n] = C::copy_offset(wave, lane, n, 0, kTile - 1, krs);
   const uint32_t smem_a = lds_at(smem);
   auto issue_tile = [&](int j) {
     const int kt = wt.tile(j);
@@ -134,13 +136,21 @@ __global__ void __launch_bounds__(256, 2) win_dq_kernel(WinBwdArgs a) {
     const char* ks = Kg + (size_t)kt * kTile * krs;
     const char* vs = Vg + (size_t)kt * kTile * vrs;
     const uint32_t dst = smem_a + (j & 1) * 2 * C::TBYTES;
+    if (lo == 0 && hi == kTile - 1 && krs == vrs) {
 #pragma unroll
-    for (int n = 0; n < C::LPW; ++n)
-      if (wave + 4 * n < C::SLOTS) {
-        const int r = clamp_row(crow[n], lo, hi);
-        dma16(__umul24(r, krs) + cchunk[n], ks, dst + 1024 * (wave + 4 * n));
-        dma16(__umul24(r, vrs) + cchunk[n], vs, dst + C::TBYTES + 1024 * (wave + 4 * n));
-      }
+      for (int n = 0; n < C::LPW; ++n)
+        if (wave + 4 * n < C::SLOTS) {
+          dma16(koff[n], ks, dst + 1024 * (wave + 4 * n));
+          dma16(koff[n], vs, dst + C::TBYTES + 1024 * (wave + 4 * n));
+        }
+    } else {
+#pragma unroll
+      for (int n = 0; n < C::LPW; ++n)
+        if (wave + 4 * n < C::SLOTS) {
+          dma16(C::copy_offset(wave, lane, n, lo, hi, krs), ks, dst + 1024 * (wave + 4 * n));
+          dma16(C::copy_offset(wave, lane, n, lo, hi, vrs), vs, dst + C::TBYTES + 1024 * (wave + 4 * n));
+        }
+    }
   };
   const uint32_t row_rd = 2 * (l32 * C::P + 8 * h);
   const int g16 = lane >> 4, s16 = lane & 15;
@@ -189,7 +199,7 @@ __global__ void __launch_bounds__(256, 2) win_dq_kernel(WinBwdArgs a) {
     f32x16 x0 = zero16(), x1 = zero16(), y0 = zero16(), y1 = zero16();
     uint32_t dS[16];
     constexpr int RING = 6;
-    auto ahead = [](int n) { return n < 2 * C::KC || D == 64 ? 5 : 4; };
+    auto ahead = [](int n) { return n < 2 * C::KC || D == 64 ? 5 : 3; };
     u32x4 ring[RING];
     auto op_of = [&](int n) -> u32x4 {
       if (n < 4 * C::KC) {
@@ -582,13 +592,11 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) win_dkdv_kernel(WinBwdAr
       wv.Vr[c] = *(const u32x4*)(vr + 16 * c);
     }
   }
-  int crow[C::LPW];
-  uint32_t cchunk[C::LPW];
+  uint32_t qoff[C::LPW], goff[C::LPW];
 #pragma unroll
-  for (int j = 0; j < C::LPW; ++j) {
-    const int t = 64 * (wave + 4 * j) + lane;
-    crow[j] = t / C::SLOTS;
-    cchunk[j] = 16 * min(t % C::SLOTS, D / 8 - 1);
+  for (int n = 0; n < C::LPW; ++n) {
+    qoff[n] = C::copy_offset(wave, lane, n, 0, kTile - 1, qrs);
+    goff[n] = C::copy_offset(wave, lane, n, 0, kTile - 1, grs);
   }
   const uint32_t smem_a = lds_at(smem);
   auto issue_tile = [&](int g, int t, int stage) {
@@ -596,13 +604,21 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) win_dkdv_kernel(WinBwdAr
     const char* qs = Qg + (size_t)t * kTile * qrs + 2 * g * D;
     const char* gs = Gg + (size_t)t * kTile * grs + 2 * g * D;
     const uint32_t dst = smem_a + stage * C::STAGE;
+    if (lo == 0 && hi == kTile - 1) {
 #pragma unroll
-    for (int n = 0; n < C::LPW; ++n)
-      if (wave + 4 * n < C::SLOTS) {
-        const int r = clamp_row(crow[n], lo, hi);
-        dma16(__umul24(r, qrs) + cchunk[n], qs, dst + 1024 * (wave + 4 * n));
-        dma16(__umul24(r, grs) + cchunk[n], gs, dst + C::TBYTES + 1024 * (wave + 4 * n));
-      }
+      for (int n = 0; n < C::LPW; ++n)
+        if (wave + 4 * n < C::SLOTS) {
+          dma16(qoff[n], qs, dst + 1024 * (wave + 4 * n));
+          dma16(goff[n], gs, dst + C::TBYTES + 1024 * (wave + 4 * n));
+        }
+    } else {
+#pragma unroll
+      for (int n = 0; n < C::LPW; ++n)
+        if (wave + 4 * n < C::SLOTS) {
+          dma16(C::copy_offset(wave, lane, n, lo, hi, qrs), qs, dst + 1024 * (wave + 4 * n));
+          dma16(C::copy_offset(wave, lane, n, lo, hi, grs), gs, dst + C::TBYTES + 1024 * (wave + 4 * n));
+        }
+    }
     if (wave == 0) {
       const float* p = a.Dsum + stat0 + (size_t)g * s.TQ + t * kTile + clamp_row(lane, lo, hi);
       dma4_v(p + stats, dst + C::STAT);

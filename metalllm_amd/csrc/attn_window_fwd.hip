@@ -12,8 +12,9 @@
 // tile j on the vector ALU between the matrix products of S of tile j + 1 and P.V of tile j - 1.
 //
 // Masks: a wave skips the tiles that none of its rows sees, and masks those that its rows see in part, before
-// the step: one unsigned compare per score, since (uint)(pos - key) < window is both the causal border and
-// the window's. The sinks add a compare in tile 0, which holds all of them and comes first.
+// the step: a compare per score with the causal border or the window's end, and where a tile has both one
+// unsigned compare, (uint)(pos - key) < window. The sinks add a compare in tile 0, which holds all of them
+// and comes first.
 //
 // The reference point m moves only when a tile's max exceeds it by 2^8 in the exponent's base (l and O
 // are fp32 and p keeps its relative precision under any reference point), so O is rarely rescaled.
@@ -96,50 +97,62 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_fwd_kernel(WinFwdArg
   for (int c = 0; c < C::KC; ++c) Qr[c] = *(const u32x4*)(Qg + 16 * c + 8 * h);
 
   // Copies: 1 KB instruction n of a tile covers 16-byte slots 64n .. 64n + 63; slot t is (row t / SLOTS,
-  // chunk t % SLOTS); pad chunks repeat the row's last chunk. Rows are held in [lo, hi], the keys that
-  // some row of the workgroup sees.
-  int krow[C::KPW], vrow[C::VPW];
-  uint32_t kchunk[C::KPW], vchunk[C::VPW];
+  // chunk t % SLOTS); pad chunks repeat the row's last chunk. Rows of a tile that [lo, hi], the keys that
+  // some row of the workgroup sees, holds in part are held in it.
+  uint32_t koff[C::KPW], voff[C::VPW];  // bytes from the tile's first row
   auto vx = [](int r) { return D == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); };
+  auto slot = [&](int n) { return 64 * (wave + 4 * n) + lane; };
+  auto koff_of = [&](int n, int lo, int hi) {
+    const int t = slot(n), r = t / C::KSLOTS;
+    return __umul24(clamp_row(r, lo, hi), krs) + 16 * min(t - r * C::KSLOTS, D / 8 - 1);
+  };
+  auto voff_of = [&](int n, int lo, int hi) {
+    const int t = slot(n), r = t / C::VSLOTS;
+    return __umul24(clamp_row(r, lo, hi), vrs) + 16 * ((t % C::VSLOTS) ^ vx(r));
+  };
 #pragma unroll
-  for (int j = 0; j < C::KPW; ++j) {
-    const int t = 64 * (wave + 4 * j) + lane;
-    krow[j] = t / C::KSLOTS;
-    kchunk[j] = 16 * min(t % C::KSLOTS, D / 8 - 1);
-  }
+  for (int n = 0; n < C::KPW; ++n) koff[n] = koff_of(n, 0, C::BN - 1);
 #pragma unroll
-  for (int j = 0; j < C::VPW; ++j) {
-    const int t = 64 * (wave + 4 * j) + lane;
-    vrow[j] = t / C::VSLOTS;
-    vchunk[j] = 16 * ((t % C::VSLOTS) ^ vx(vrow[j]));
-  }
+  for (int n = 0; n < C::VPW; ++n) voff[n] = voff_of(n, 0, C::BN - 1);
   const uint32_t smem_a = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)smem;
+  // the rows of step j's tile that may be read; whether that is all of them
   auto rows_of = [&](int j, int kt, int& lo, int& hi) {
     const bool sink_tile = j < wt.sink;
     lo = sink_tile ? 0 : max(wt.lo - kt * C::BN, 0);
     hi = sink_tile ? s.sinks - 1 : min(wt.hi - kt * C::BN, C::BN - 1);
+    return lo == 0 && hi == C::BN - 1;
   };
   auto load_k = [&](int j, int stage) {
     const int kt = wt.tile(j);
     int lo, hi;
-    rows_of(j, kt, lo, hi);
+    const bool all = rows_of(j, kt, lo, hi);
     const char* src = Kg + (size_t)kt * C::BN * krs;
     const uint32_t dst = smem_a + stage * C::STAGE;
+    if (all) {
 #pragma unroll
-    for (int n = 0; n < C::KPW; ++n)
-      if (wave + 4 * n < C::KSLOTS)
-        dma16(__umul24(clamp_row(krow[n], lo, hi), krs) + kchunk[n], src, dst + 1024 * (wave + 4 * n));
+      for (int n = 0; n < C::KPW; ++n)
+        if (wave + 4 * n < C::KSLOTS) dma16(koff[n], src, dst + 1024 * (wave + 4 * n));
+    } else {
+#pragma unroll
+      for (int n = 0; n < C::KPW; ++n)
+        if (wave + 4 * n < C::KSLOTS) dma16(koff_of(n, lo, hi), src, dst + 1024 * (wave + 4 * n));
+    }
   };
   auto load_v = [&](int j, int stage) {
     const int kt = wt.tile(j);
     int lo, hi;
-    rows_of(j, kt, lo, hi);
+    const bool all = rows_of(j, kt, lo, hi);
     const char* src = Vg + (size_t)kt * C::BN * vrs;
     const uint32_t dst = smem_a + stage * C::STAGE + C::KBYTES;
+    if (all) {
 #pragma unroll
-    for (int n = 0; n < C::VPW; ++n)
-      if (wave + 4 * n < C::VSLOTS)
-        dma16(__umul24(clamp_row(vrow[n], lo, hi), vrs) + vchunk[n], src, dst + 1024 * (wave + 4 * n));
+      for (int n = 0; n < C::VPW; ++n)
+        if (wave + 4 * n < C::VSLOTS) dma16(voff[n], src, dst + 1024 * (wave + 4 * n));
+    } else {
+#pragma unroll
+      for (int n = 0; n < C::VPW; ++n)
+        if (wave + 4 * n < C::VSLOTS) dma16(voff_of(n, lo, hi), src, dst + 1024 * (wave + 4 * n));
+    }
   };
 
   // LDS operand bases (elements inside a stage). K rows: A operand of S^T, lane = key row. V^T by
@@ -197,7 +210,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_fwd_kernel(WinFwdArg
       const int t = n - NPV;
       return lds_read16(kb + (t & 1) * 32 * C::KP + 16 * (t >> 1));
     };
-    constexpr int RING = D == 64 ? 4 : 6;
+    constexpr int RING = D == 64 ? 3 : 6;
     u32x4 ring[RING];
 #pragma unroll
     for (int n = 0; n < RING - 1; ++n)
@@ -302,19 +315,31 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_fwd_kernel(WinFwdArg
   const bool active = i0 + 32 * wave <= i1 && pw1 >= 0;
   const int jw0 = !active ? n + 1 : s.sinks > 0 ? 0 : max(0, pw0 - s.window + 1) / C::BN + j_of;
   const int jw1 = active ? pw1 / C::BN + j_of : -1;
-  auto mask = [&](auto first, int j, f32x16& X0, f32x16& X1) __attribute__((always_inline)) {
-    const int ka = wt.tile(j) * C::BN;
-    if (ka + C::BN - 1 <= pw0 && pw0 + 31 - ka < s.window) return;  // seen whole
-    int dq = pos - ka - 4 * h;  // score r of half t is key ka + 4h + off
-    asm volatile("" : "+v"(dq));  // (opaque: 32 loop-invariant bounds would be kept instead)
-    // keys ka + 4h + off < sinks: the sinks are in tile 0, and that is the wave's first one then
-    const int few = decltype(first)::value ? min(s.sinks - ka - 4 * h, dq + 1) : 0;
+  auto hide = [&](f32x16& X0, f32x16& X1, auto seen) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < 32; ++e) {
-      const int off = 32 * (e >> 4) + 8 * ((e & 15) >> 2) + (e & 3);
       f32x16& X = e < 16 ? X0 : X1;
-      const bool seen = (uint32_t)(dq - off) < (uint32_t)s.window || (decltype(first)::value && off < few);
-      X[e & 15] = seen ? X[e & 15] : -INFINITY;
+      X[e & 15] = seen(32 * (e >> 4) + 8 * ((e & 15) >> 2) + (e & 3)) ? X[e & 15] : -INFINITY;
+    }
+  };
+  auto mask = [&](auto first, int j, f32x16& X0, f32x16& X1) __attribute__((always_inline)) {
+    const int ka = wt.tile(j) * C::BN;
+    const bool all_before = ka + C::BN - 1 <= pw0, all_inside = pw0 + 31 - ka < s.window;
+    if (all_before && all_inside) return;
+    int dq = pos - ka - 4 * h;  // score e is of key ka + 4h + off
+    asm volatile("" : "+v"(dq));  // (opaque: 32 loop-invariant bounds would be kept instead)
+    const uint32_t window = s.window;
+    if (decltype(first)::value) {
+      // keys ka + 4h + off < sinks: the sinks are in tile 0, and that is the wave's first one then
+      const int few = min(s.sinks - ka - 4 * h, dq + 1);
+      hide(X0, X1, [&](int off) { return (uint32_t)(dq - off) < window || off < few; });
+    } else if (all_inside) {  // the border alone
+      hide(X0, X1, [&](int off) { return off <= dq; });
+    } else if (all_before) {  // the window's end alone
+      const int end = dq - s.window;
+      hide(X0, X1, [&](int off) { return off > end; });
+    } else {
+      hide(X0, X1, [&](int off) { return (uint32_t)(dq - off) < window; });
     }
   };
   int j = 0;
