@@ -101,13 +101,14 @@ inline size_t win_token_floats(const WinShape& s, int D, int splits) {
   const size_t tiles = ((size_t)s.TQ * s.G + kTokRows - 1) / kTokRows;
   return splits > 1 ? (size_t)s.B * s.NKV * tiles * splits * kTokRows * (D + 2) : 0;
 }
-// Parts that the query tiles beyond the window of the sink keys' block are dealt to (0: there are none).
+// Parts that the query tiles (of all heads of a group) beyond the windows of the sink keys' block are dealt to
+// (0: there are none), a few tiles each: they run last, in the gaps that the key blocks leave.
+constexpr int kSinkTiles = 4, kSinkSplits = 128;
 inline int win_sink_splits(const WinShape& s) {
   const int64_t far = (int64_t)s.TK - (kBwdBlockN - 1) - s.window;  // rows that see the sinks alone of block 0
   if (s.sinks == 0 || far <= 0) return 0;
-  const int64_t usual = ((int64_t)s.window + kBwdBlockN - 1) / kTile + 1, tiles = (far + kTile - 1) / kTile;
-  const int64_t n = (tiles + usual - 1) / usual;
-  return (int)(n < 64 ? n : 64);
+  const int64_t n = (s.G * ((far + kTile - 1) / kTile) + kSinkTiles - 1) / kSinkTiles;
+  return (int)(n < kSinkSplits ? n : kSinkSplits);
 }
 inline size_t win_sink_floats(const WinShape& s, int D, int splits) {
   return splits ? (size_t)s.B * s.NKV * (splits + 1) * 2 * kWinMaxSinks * D : 0;

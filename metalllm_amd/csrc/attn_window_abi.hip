@@ -28,7 +28,7 @@ int validate(const metalllmWindowParams* p) {
   if (p->B == 0 || p->NH == 0 || p->NKV == 0 || p->NH % p->NKV) return METALLLM_ATTN_E_LAYOUT;
   if (p->window == 0 || p->sinks > mla::kWinMaxSinks) return METALLLM_ATTN_E_WINDOW;
   if (p->TQ > kMostRows || p->TK > kMostRows) return METALLLM_ATTN_E_SIZE;
-  const uint64_t blocks = (uint64_t)(p->TQ > p->TK ? p->TQ : p->TK) / 64 + 65;
+  const uint64_t blocks = (uint64_t)(p->TQ > p->TK ? p->TQ : p->TK) / 64 + 129;
   if ((uint64_t)p->B * p->NH > (1u << 24) || (uint64_t)p->B * p->NH * blocks >= (1ull << 31)) return METALLLM_ATTN_E_SIZE;
   if (!strides_ok(*p, p->TQ, p->NH, p->q_row, p->q_seq) || !strides_ok(*p, p->TK, p->NKV, p->k_row, p->k_seq) ||
       !strides_ok(*p, p->TK, p->NKV, p->v_row, p->v_seq) || !strides_ok(*p, p->TQ, p->NH, p->o_row, p->o_seq))

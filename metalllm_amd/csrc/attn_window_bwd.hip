@@ -80,7 +80,7 @@ struct IntTag {
 // ---- dQ: query owner ----
 
 template <int D>
-__global__ void __launch_bounds__(256, 2) win_dq_kernel(WinBwdArgs a) {
+__global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_dq_kernel(WinBwdArgs a) {
   using C = WbCfg<D>;
   constexpr int BM = kDqBlockM;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * C::TBYTES];
@@ -413,7 +413,10 @@ struct WinKeyWave {
 
   // Query rows staged at LDS byte address stage_a; MASK: row r of the tile (position p0 + r) sees the lane's
   // key where (uint)(p0 + r - key) < lim; d0 = p0 + 4h - key. Slots (one product each):
-  //   [0, KC) S of rows 0-31  [KC, 2KC) dP  [2KC, 3KC) S of rows 32-63  [3KC, 4KC) dP  then 4 per chain
+  //   [0, 2KC) S and dP of rows 0-31 in turn, [2KC, 4KC) of rows 32-63, then dV and dK, 16 rows at a time over
+  //   the d tiles: two products that follow each other never add to the same sum, since the second would
+  //   wait for the first to leave the matrix core
+  // Beside them p, then dS, of rows 0-31 from slot 2KC, of rows 32-63 from slot 4KC.
   template <bool MASK>
   __device__ __forceinline__ void step(uint32_t stage_a, int d0, uint32_t lim) {
     constexpr int NS = 4 * C::KC + 8 * C::DT;
@@ -427,33 +430,24 @@ struct WinKeyWave {
     uint32_t Pp[16], dS[16];
     auto operand = [&](int i) -> u32x4 {
       if (i < 4 * C::KC) {
-        const int seg = i / C::KC, t = seg >> 1, c = i % C::KC;
-        return lds_b128_w(row_a + ((seg & 1) ? C::TBYTES : 0) + 2 * (32 * t * C::P + 16 * c));
+        const int t = i / (2 * C::KC), c = (i % (2 * C::KC)) >> 1;
+        return lds_b128_w(row_a + ((i & 1) ? C::TBYTES : 0) + 2 * (32 * t * C::P + 16 * c));
       }
-      const int k = i - 4 * C::KC, n = k / 4, j = k % 4, dt = n % C::DT;
-      const uint32_t src = tr_a + (n >= C::DT ? 0 : C::TBYTES) + 2 * (16 * j * C::P + 32 * dt);
+      const int k = i - 4 * C::KC, j = k / C::DT % 4, dt = k % C::DT;
+      const uint32_t src = tr_a + (k >= 4 * C::DT ? 0 : C::TBYTES) + 2 * (16 * j * C::P + 32 * dt);
       const u32x2 lo = lds_tr_w(src), hi = lds_tr_w(src + 2 * 8 * C::P);
       return u32x4{lo[0], lo[1], hi[0], hi[1]};
     };
+    // vector work in slot i: kind 1 = p, 2 = dS of pairs u0 .. of half t; PPS pairs to a slot
     struct Work {
       int kind, t, u0, cnt;
     };
-    // pairs of vector work in slot i: kind 1 = p of half t, 2 = dS of half t
     auto work = [&](int i) -> Work {
-      if (i < 4 * C::KC) {
-        const int seg = i / C::KC, u0 = (i % C::KC) * PPS;
-        if (seg == 1) return {1, 0, u0, PPS};
-        if (seg == 2) return {2, 0, u0, PPS};
-        if (seg == 3) return {1, 1, u0, PPS};
-        return {0, 0, 0, 0};
-      }
-      const int k = i - 4 * C::KC;
-      if (k < 4 * C::DT) {
-        constexpr int SPAN = (4 * C::DT) / 8;
-        if (k % SPAN == 0) return {2, 1, k / SPAN, 1};
-      }
-      return {0, 0, 0, 0};
+      if (i < 2 * C::KC || i >= 6 * C::KC) return {0, 0, 0, 0};
+      const int t = i >= 4 * C::KC, n = (i - (t ? 4 : 2) * C::KC) * PPS;
+      return n < 8 ? Work{1, t, n, PPS} : Work{2, t, n - 8, PPS};
     };
+    static_assert(C::KC == 2 * C::DT, "slots of a half's vector work");
     auto stats = [&](int i) -> f32x4 {
       const Work w = work(i);
       const uint32_t ad = stat_a + (w.kind == 2 ? 256 : 0) + 4 * (32 * w.t + 8 * (w.u0 >> 1) + 2 * (w.u0 & 1));
@@ -499,13 +493,16 @@ struct WinKeyWave {
       if (i + SA < NS && work(i + SA).kind) sring[(i + SA) % (SA + 1)] = stats(i + SA);
       const u32x4& op = ring[i % RING];
       if (i < 4 * C::KC) {
-        const int seg = i / C::KC, c = i % C::KC;
-        if (seg == 0) x0 = mfma(op, Kr[c], x0);
-        else if (seg == 1) y0 = mfma(op, Vr[c], y0);
-        else if (seg == 2) x1 = mfma(op, Kr[c], x1);
-        else y1 = mfma(op, Vr[c], y1);
+        const int t = i / (2 * C::KC), c = (i % (2 * C::KC)) >> 1;
+        if (i & 1) {
+          if (t) y1 = mfma(op, Vr[c], y1);
+          else y0 = mfma(op, Vr[c], y0);
+        } else {
+          if (t) x1 = mfma(op, Kr[c], x1);
+          else x0 = mfma(op, Kr[c], x0);
+        }
       } else {
-        const int k = i - 4 * C::KC, n = k / 4, j = k % 4;
+        const int k = i - 4 * C::KC, j = k / C::DT % 4, n = k % C::DT + (k >= 4 * C::DT ? C::DT : 0);
         const uint32_t* src = n >= C::DT ? dS : Pp;
         st[n] = mfma(op, u32x4{src[4 * j], src[4 * j + 1], src[4 * j + 2], src[4 * j + 3]}, st[n]);
       }
@@ -535,11 +532,16 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) win_dkdv_kernel(WinBwdAr
   const int h = lane >> 5, l32 = lane & 31;
   const WinShape& s = a.s;
   const int nkb = (s.TK + BN - 1) / BN;
+  // the key blocks first, then (far) the parts of the rows that see block 0's sinks alone
+  const int groups = s.B * s.NKV, near = groups * nkb;
+  const bool far = (int)blockIdx.x >= near;
   int group, blk;
-  decode_workgroup(blockIdx.x, s.B * s.NKV, nkb + a.splits, false, kBwdDispatchRound, group, blk);
+  if (far)
+    decode_workgroup(blockIdx.x - near, groups, a.splits, false, kBwdDispatchRound, group, blk);
+  else
+    decode_workgroup(blockIdx.x, groups, nkb, false, kBwdDispatchRound, group, blk);
   const int b = group / s.NKV, kvh = group - b * s.NKV;
-  const bool far = blk < a.splits;  // a part of the rows that see block 0's sinks alone
-  const int kb = far ? 0 : blk - a.splits;
+  const int kb = far ? 0 : blk;
   const WinSeq sq = win_seq(s, b);
   const int k0 = kb * BN;
   const bool split = kb == 0 && a.splits > 0;  // sink keys go through the workspace
@@ -747,22 +749,29 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) win_dkdv_kernel(WinBwdAr
     }
 }
 
-// dK, dV of the sink keys: one workgroup per (sequence, key head), a thread per four columns of a row.
+// dK, dV of the sink keys: a workgroup per (sequence, key head) and key; 8 threads to four columns, each with
+// every 8th part, joined in order.
 template <int D>
-__global__ void __launch_bounds__(256) win_sink_kernel(WinBwdArgs a) {
+__global__ void __launch_bounds__(D * 4) win_sink_kernel(WinBwdArgs a) {
+  __shared__ f32x4 sums[8][D / 2];
   const WinShape& s = a.s;
-  const int group = blockIdx.x, b = group / s.NKV, kvh = group - b * s.NKV;
-  const int keys = min(s.sinks, win_seq(s, b).lk);
-  const float* in = a.part + (size_t)group * (a.splits + 1) * 2 * kWinMaxSinks * D;
-  for (int t = threadIdx.x; t < 2 * keys * (D / 4); t += 256) {
-    const int c = t % (D / 4), r = t / (D / 4), key = r >> 1, isv = r & 1;
-    const float* p = in + (size_t)isv * kWinMaxSinks * D + key * D + 4 * c;
-    f32x4 sum = *(const f32x4*)p;
-    for (int v = 1; v <= a.splits; ++v) sum += *(const f32x4*)(p + (size_t)v * 2 * kWinMaxSinks * D);
-    if (!isv) sum *= s.scale;
-    uint16_t* o = isv ? a.dV + b * s.v_seq + (size_t)key * s.v_row : a.dK + b * s.k_seq + (size_t)key * s.k_row;
-    *(u32x2*)(o + kvh * D + 4 * c) = u32x2{pack_bf16(sum[0], sum[1]), pack_bf16(sum[2], sum[3])};
-  }
+  const int group = blockIdx.x / s.sinks, key = blockIdx.x - group * s.sinks;
+  const int b = group / s.NKV, kvh = group - b * s.NKV;
+  if (key >= win_seq(s, b).lk) return;
+  const int t = threadIdx.x % (D / 2), w = threadIdx.x / (D / 2), isv = t / (D / 4), c = 4 * (t % (D / 4));
+  const size_t step = (size_t)2 * kWinMaxSinks * D;
+  const float* in = a.part + (size_t)group * (a.splits + 1) * step + (size_t)isv * kWinMaxSinks * D + key * D + c;
+  f32x4 sum = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int v = w; v <= a.splits; v += 8) sum += *(const f32x4*)(in + v * step);
+  sums[w][t] = sum;
+  __syncthreads();
+  if (w) return;
+#pragma unroll
+  for (int v = 1; v < 8; ++v) sum += sums[v][t];
+  if (!isv) sum *= s.scale;
+  uint16_t* o = isv ? a.dV + b * s.v_seq + (size_t)key * s.v_row : a.dK + b * s.k_seq + (size_t)key * s.k_row;
+  *(u32x2*)(o + kvh * D + c) = u32x2{pack_bf16(sum[0], sum[1]), pack_bf16(sum[2], sum[3])};
 }
 
 hipError_t launch_window_backward(const WinBwdArgs& a, int D, hipStream_t s) {
@@ -776,7 +785,7 @@ hipError_t launch_window_backward(const WinBwdArgs& a, int D, hipStream_t s) {
   hipLaunchKernelGGL((D == 64 ? win_dkdv_kernel<64> : win_dkdv_kernel<128>), dim3(nk), dim3(256), 0, s, a);
   e = hipGetLastError();
   if (e != hipSuccess || a.splits == 0) return e;
-  hipLaunchKernelGGL((D == 64 ? win_sink_kernel<64> : win_sink_kernel<128>), dim3(groups), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((D == 64 ? win_sink_kernel<64> : win_sink_kernel<128>), dim3(groups * p.sinks), dim3(D * 4), 0, s, a);
   return hipGetLastError();
 }
 

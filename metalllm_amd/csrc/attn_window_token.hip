@@ -14,7 +14,7 @@
 // A step takes 32 keys. Its K registers are loaded again as soon as its scores are formed, its V registers
 // as soon as its products are; the loads of three waves per SIMD cover the rest.
 //
-// Split: the steps are dealt to the 4 waves of a workgroup, and over `splits` workgroups where there are
+// Split: the steps are dealt to the waves of a workgroup, and over `splits` workgroups where there are
 // too few (sequence, key head) pairs to fill the chip; each part keeps its own reference point and sum, and
 // they are joined in LDS, or through the workspace by a second small kernel.
 #include <algorithm>
@@ -75,11 +75,12 @@ __device__ __forceinline__ WtRange wt_range(const WinShape& s, const WinSeq& q, 
 
 // SEVERAL: more than one query row (TQ > 1), which may see different keys of a step; its path for values that
 // are not finite takes registers that one row does without.
-template <int D, bool SEVERAL>
-__global__ void __launch_bounds__(256, SEVERAL ? 2 : D == 64 ? 4 : 3) win_token_kernel(WinFwdArgs a) {
+// WAVES: 4, or 8 where there are so few units that their keys are better split inside one workgroup.
+template <int D, bool SEVERAL, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || SEVERAL ? 2 : D == 64 ? 4 : 3) win_token_kernel(WinFwdArgs a) {
   using C = WtCfg<D>;
-  __shared__ __attribute__((aligned(16))) float sm_o[4][kTokRows][C::PITCH];
-  __shared__ float sm_m[4][kTokRows], sm_l[4][kTokRows];
+  __shared__ __attribute__((aligned(16))) float sm_o[WAVES][kTokRows][C::PITCH];
+  __shared__ float sm_m[WAVES][kTokRows], sm_l[WAVES][kTokRows];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, n16 = lane & 15;
@@ -91,7 +92,7 @@ __global__ void __launch_bounds__(256, SEVERAL ? 2 : D == 64 ? 4 : 3) win_token_
   const WinSeq sq = win_seq(s, b);
   const WtRange w = wt_range(s, sq, rt);
   if (w.i_lo > w.i_hi) return;  // rows behind the sequence: left as they were (the join too)
-  const int parts = 4 * a.splits, part = 4 * split + wave;
+  const int parts = WAVES * a.splits, part = WAVES * split + wave;
   const int t0 = (int)((int64_t)w.steps * part / parts), t1 = (int)((int64_t)w.steps * (part + 1) / parts);
 
   const int row = rt * kTokRows + n16, qi = row / s.G;
@@ -251,14 +252,15 @@ __global__ void __launch_bounds__(256, SEVERAL ? 2 : D == 64 ? 4 : 3) win_token_
     for (int e = 0; e < C::E; ++e) sm_o[wave][n16][C::E * (4 * g + r) + e] = O[e][r];
   __syncthreads();
   const int jr = tid >> 4, d0 = (tid & 15) * C::E;  // row and columns that this thread joins
+  if (jr >= kTokRows) return;
   float M = -INFINITY;
 #pragma unroll
-  for (int v = 0; v < 4; ++v) M = fmaxf(M, sm_m[v][jr]);
+  for (int v = 0; v < WAVES; ++v) M = fmaxf(M, sm_m[v][jr]);
   float L = 0.0f, acc[C::E];
 #pragma unroll
   for (int e = 0; e < C::E; ++e) acc[e] = 0.0f;
 #pragma unroll
-  for (int v = 0; v < 4; ++v) {
+  for (int v = 0; v < WAVES; ++v) {
     const float m = sm_m[v][jr];
     if (m == -INFINITY && sm_l[v][jr] == 0.0f) continue;  // a part without visible keys
     const float f = exp2_hw(m - (M == -INFINITY ? 0.0f : M));
@@ -326,28 +328,39 @@ __global__ void __launch_bounds__(256) win_join_kernel(WinFwdArgs a) {
     a.l[((size_t)b * s.NH + head) * s.TQ + qi] = empty ? -INFINITY : M * (1.0f / kLog2e) + logf(L);
 }
 
-// Workgroups per (sequence, key head, row tile): enough for three per CU, each wave keeping two steps or more.
+// Waves to a workgroup and workgroups to a unit (sequence, key head, row tile), from the steps that a unit
+// has at most. A workgroup per unit joins its waves in LDS; more of them take a second kernel (about 5 us), so
+// they are for units that are too few to fill the chip and have steps enough for 6 to a wave.
+static int64_t token_units(const WinShape& s) {
+  return (int64_t)s.B * s.NKV * (((int64_t)s.TQ * s.G + kTokRows - 1) / kTokRows);
+}
+static int token_waves(const WinShape& s) { return token_units(s) <= kCus / 2 ? 8 : 4; }
 int win_token_splits(const WinShape& s) {
-  const int64_t units = (int64_t)s.B * s.NKV * (((int64_t)s.TQ * s.G + kTokRows - 1) / kTokRows);
+  const int64_t units = token_units(s), waves = token_waves(s);
   const int64_t keys = std::min<int64_t>((int64_t)s.window + s.TQ - 1, s.TK) + s.sinks;
   const int64_t steps = (keys + 31) / 32;
-  const int64_t want = std::min<int64_t>((3 * kCus + units - 1) / units, steps / 8);
+  const int64_t fill = 12 * kCus / waves;  // workgroups resident at once
+  const int64_t want = std::min<int64_t>((fill + units - 1) / units, steps / (6 * waves));
   return (int)std::max<int64_t>(1, std::min<int64_t>(want, 64));
 }
 
-hipError_t launch_window_token(const WinFwdArgs& a, int D, hipStream_t s) {
-  const unsigned units = (unsigned)(a.s.B * a.s.NKV * ((a.s.TQ * a.s.G + kTokRows - 1) / kTokRows));
+template <int D>
+static hipError_t launch_token(const WinFwdArgs& a, unsigned units, hipStream_t s) {
   const bool several = a.s.TQ > 1;
-  auto kernel = D == 64 ? (several ? win_token_kernel<64, true> : win_token_kernel<64, false>)
-                        : (several ? win_token_kernel<128, true> : win_token_kernel<128, false>);
-  hipLaunchKernelGGL(kernel, dim3(units * a.splits), dim3(256), 0, s, a);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.splits == 1) return e;
-  if (D == 64)
-    hipLaunchKernelGGL(win_join_kernel<64>, dim3(units), dim3(256), 0, s, a);
+  const dim3 grid(units * a.splits);
+  if (token_waves(a.s) == 8)
+    hipLaunchKernelGGL((several ? win_token_kernel<D, true, 8> : win_token_kernel<D, false, 8>), grid, dim3(512), 0, s, a);
   else
-    hipLaunchKernelGGL(win_join_kernel<128>, dim3(units), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((several ? win_token_kernel<D, true, 4> : win_token_kernel<D, false, 4>), grid, dim3(256), 0, s, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.splits == 1) return e;
+  hipLaunchKernelGGL(win_join_kernel<D>, dim3(units), dim3(256), 0, s, a);
   return hipGetLastError();
+}
+
+hipError_t launch_window_token(const WinFwdArgs& a, int D, hipStream_t s) {
+  const unsigned units = (unsigned)token_units(a.s);
+  return D == 64 ? launch_token<64>(a, units, s) : launch_token<128>(a, units, s);
 }
 
 }  // namespace mla
