@@ -7,6 +7,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "attn_common.hpp"
 #include "attn_launch.hpp"
 
 namespace mla {
@@ -84,6 +85,34 @@ __device__ __forceinline__ WinTiles win_tiles(const WinShape& s, const WinSeq& q
 
 // Rows of one head as the query side of a workgroup or the key side of another see them.
 __device__ __forceinline__ int clamp_row(int r, int lo, int hi) { return min(max(r, lo), hi); }
+
+// A wave's 32 rows x D outputs, held as accumulators (lane: row l32, values 32 dt + 8g + 4h + 0..3 in registers
+// 4g .. of acc[dt]) -> bf16 rows in memory, through LDS: a lane stores 16 bytes of a row, 64 lanes whole
+// rows. Straight from the registers it is twice the instructions, each over 32 rows.
+// lds: kRowsOut<D> bytes of the wave's own; live(r): whether row r is written.
+template <int D>
+constexpr int kRowsOut = 32 * (2 * D + 16);
+template <int D, class Acc, class Live>
+__device__ __forceinline__ void store_rows(uint32_t lds, int lane, const Acc* acc, float scale, uint16_t* out, uint32_t row,
+                                           Live live) {
+  typedef uint32_t v2 __attribute__((ext_vector_type(2)));
+  typedef uint32_t v4 __attribute__((ext_vector_type(4)));
+  constexpr uint32_t P = 2 * D + 16;
+  const int h = lane >> 5, l32 = lane & 31;
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *(__attribute__((address_space(3))) v2*)(uintptr_t)(lds + l32 * P + 64 * dt + 16 * g + 8 * h) =
+          v2{pack_bf16(acc[dt][4 * g] * scale, acc[dt][4 * g + 1] * scale),
+             pack_bf16(acc[dt][4 * g + 2] * scale, acc[dt][4 * g + 3] * scale)};
+#pragma unroll
+  for (int n = 0; n < D / 16; ++n) {
+    const int t = 64 * n + lane, r = t / (D / 8), c = t % (D / 8);
+    const v4 x = *(const __attribute__((address_space(3))) v4*)(uintptr_t)(lds + r * P + 16 * c);
+    if (live(r)) *(v4*)(out + (size_t)r * row + 8 * c) = x;
+  }
+}
 
 // Whether query position `pos` sees key j.
 __device__ __forceinline__ bool win_sees(const WinShape& s, int pos, int j) {

@@ -58,12 +58,29 @@ struct WbCfg {
   static constexpr int STAGE = 2 * TBYTES + 512;
   static constexpr int KC = D / 16;
   static constexpr int DT = D / 32;
-  // Byte offset, from a tile's first row, of what the lane copies in the wave's instruction n: 16-byte slot t
-  // of the padded tile, row t / SLOTS held in [lo, hi], pad chunks repeating the row's last one.
-  __device__ static __forceinline__ uint32_t copy_offset(int wave, int lane, int n, int lo, int hi, uint32_t row_bytes) {
-    const int t = 64 * (wave + 4 * n) + lane, r = t / SLOTS;
-    return __umul24(clamp_row(r, lo, hi), row_bytes) + 16 * min(t - r * SLOTS, D / 8 - 1);
-  }
+  // What a lane copies of a tile's rows: instruction n of the wave covers 16-byte slots 64 (wave + 4n) .. + 63 of
+  // the padded tile; slot t is row t / SLOTS, chunk t % SLOTS, pad chunks repeating the row's last one. Part
+  // n copies that of two tensors, whose rows are held in [lo, hi].
+  struct Slots {
+    int wave, row[LPW];
+    uint32_t chunk[LPW];
+    __device__ __forceinline__ Slots(int wave_, int lane) : wave(wave_) {
+#pragma unroll
+      for (int n = 0; n < LPW; ++n) {
+        const int t = 64 * (wave + 4 * n) + lane;
+        row[n] = t / SLOTS;
+        chunk[n] = 16 * min(t % SLOTS, D / 8 - 1);
+      }
+    }
+    __device__ __forceinline__ void copy(int n, int lo, int hi, const char* a, uint32_t a_row, const char* b, uint32_t b_row,
+                                         uint32_t dst) const {
+      if (wave + 4 * n < SLOTS) {
+        const int r = clamp_row(row[n], lo, hi);
+        dma16(__umul24(r, a_row) + chunk[n], a, dst + 1024 * (wave + 4 * n));
+        dma16(__umul24(r, b_row) + chunk[n], b, dst + TBYTES + 1024 * (wave + 4 * n));
+      }
+    }
+  };
 };
 
 // Most tiles of a query block whose rows' Dl is summed over the keys: up to here some row sees 128 keys or
@@ -101,7 +118,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_dq_kernel(WinBwdArgs
   const int i = i0 + 32 * wave + l32, ic = min(i, i1);
   const bool row_ok = i <= i1;
   const int pos = sq.off + i;
-  uint16_t* dQg = a.dQ + b * s.q_seq + (size_t)ic * s.q_row + head * D;
+  uint16_t* dQg = a.dQ + b * s.q_seq + (size_t)(i0 + 32 * wave) * s.q_row + head * D;  // the wave's rows
   const size_t stat = ((size_t)b * s.NH + head) * s.TQ + ic, stats = (size_t)s.B * s.NH * s.TQ;
 
   // Q^T and dO^T as B operands: lane holds the row, d = 16c + 8h .. +7. Dl from dO and the rounded O: half a
@@ -123,35 +140,24 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_dq_kernel(WinBwdArgs
   const char* Kg = (const char*)(a.k + b * s.k_seq + kvh * D);
   const char* Vg = (const char*)(a.v + b * s.v_seq + kvh * D);
   const uint32_t krs = 2 * s.k_row, vrs = 2 * s.v_row;
-  // bytes of the copies' rows from the tile's first (attn_window_fwd.hip)
-  uint32_t koff[C::LPW];  // k's, and v's where its rows are as far apart
-#pragma unroll
-  for (int n = 0; n < C::LPW; ++n) koff[n] = C::copy_offset(wave, lane, n, 0, kTile - 1, krs);
+  // Copies of the tile aimed at, in C::LPW parts that a step issues among its products (attn_window_fwd.hip)
+  const typename C::Slots cp(wave, lane);
   const uint32_t smem_a = lds_at(smem);
-  auto issue_tile = [&](int j) {
+  const char *ks = Kg + (size_t)wt.tile(0) * kTile * krs, *vs = Vg + (size_t)wt.tile(0) * kTile * vrs;
+  int lo = 0, hi = 0;
+  uint32_t dst = 0;
+  auto aim = [&](int j) {
     const int kt = wt.tile(j);
-    const bool sink_tile = j < wt.sink;
-    const int lo = sink_tile ? 0 : max(wt.lo - kt * kTile, 0);
-    const int hi = sink_tile ? s.sinks - 1 : min(wt.hi - kt * kTile, kTile - 1);
-    const char* ks = Kg + (size_t)kt * kTile * krs;
-    const char* vs = Vg + (size_t)kt * kTile * vrs;
-    const uint32_t dst = smem_a + (j & 1) * 2 * C::TBYTES;
-    if (lo == 0 && hi == kTile - 1 && krs == vrs) {
-#pragma unroll
-      for (int n = 0; n < C::LPW; ++n)
-        if (wave + 4 * n < C::SLOTS) {
-          dma16(koff[n], ks, dst + 1024 * (wave + 4 * n));
-          dma16(koff[n], vs, dst + C::TBYTES + 1024 * (wave + 4 * n));
-        }
-    } else {
-#pragma unroll
-      for (int n = 0; n < C::LPW; ++n)
-        if (wave + 4 * n < C::SLOTS) {
-          dma16(C::copy_offset(wave, lane, n, lo, hi, krs), ks, dst + 1024 * (wave + 4 * n));
-          dma16(C::copy_offset(wave, lane, n, lo, hi, vrs), vs, dst + C::TBYTES + 1024 * (wave + 4 * n));
-        }
+    if (j > 0) {
+      const int64_t rows = (int64_t)kTile * (kt - wt.tile(j - 1));
+      ks += rows * krs;
+      vs += rows * vrs;
     }
+    lo = j < wt.sink ? 0 : max(wt.lo - kt * kTile, 0);
+    hi = j < wt.sink ? s.sinks - 1 : min(wt.hi - kt * kTile, kTile - 1);
+    dst = smem_a + (j & 1) * 2 * C::TBYTES;
   };
+  auto part = [&](int n) __attribute__((always_inline)) { cp.copy(n, lo, hi, ks, krs, vs, vrs, dst); };
   const uint32_t row_rd = 2 * (l32 * C::P + 8 * h);
   const int g16 = lane >> 4, s16 = lane & 15;
   const uint32_t tr_rd = 2 * ((4 * h + (s16 >> 2)) * C::P + 16 * (g16 & 1) + 4 * (s16 & 3));
@@ -183,7 +189,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_dq_kernel(WinBwdArgs
     }
   };
   constexpr int NM = 4 * C::KC + 4 * C::DT, NV = Sched::dq_slot(4 * C::DT - 1) + 1;
-  auto tile = [&](int j, auto mask_tag) __attribute__((always_inline)) {
+  auto tile = [&](int j, auto mask_tag, auto part) __attribute__((always_inline)) {
     constexpr int MASK = decltype(mask_tag)::value;
     const uint32_t kb = smem_a + (j & 1) * 2 * C::TBYTES, vb = kb + C::TBYTES;
     int dq = 0, sq_ = 0;
@@ -243,6 +249,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_dq_kernel(WinBwdArgs
     };
 #pragma unroll
     for (int slot = 0; slot < NV; ++slot) {
+      if ((slot & 1) && slot / 2 < C::LPW) part(slot / 2);
       const int n = Sched::product_at(slot);
       if (n >= 0) {
 #pragma unroll
@@ -274,26 +281,28 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_dq_kernel(WinBwdArgs
     }
   };
 
-  // How the wave's rows see the tile of step j: not at all (0), in part (1), or every row every key (2)
+  // The wave's rows [pw0, pw1] (positions) see tiles of the steps jv0 .. jv1 - 1 (and the sinks in step 0), and
+  // those of jw0 .. jw1 - 1 whole: every row every key
   const int pw0 = sq.off + i0 + 32 * wave, pw1 = min(pw0 + 31, sq.off + i1);
-  auto sight = [&](int j) {
-    const int ka = wt.tile(j) * kTile;
-    if (i0 + 32 * wave > i1 || ka > pw1 || (ka + kTile - 1 <= pw0 - s.window && (ka > 0 || s.sinks == 0))) return 0;
-    return ka + kTile - 1 <= pw0 && pw1 - ka < s.window ? 2 : 1;
-  };
+  const int j_of = wt.sink - wt.t0;  // step of window tile kt: kt + j_of
+  const bool active = i0 + 32 * wave <= i1 && pw1 >= 0;
+  const int jv0 = active ? max(0, pw0 - s.window + 1) / kTile + j_of : wt.n, jv1 = active ? pw1 / kTile + j_of + 1 : 0;
+  const int jw0 = (max(0, pw1 - s.window + 1) + kTile - 1) / kTile + j_of, jw1 = max(0, pw0 + 1) / kTile + j_of;
+  const bool sinks = active && s.sinks > 0;
 
   // Rows of few keys: there the rounding of O is of the size of dP itself, so Dl = sum_j P_ij dP_ij, in a pass
   // over the tiles of its own (two of the three products again).
   if (wt.n <= kExactTiles) {
     dl = 0.0f;
     for (int j = 0; j < wt.n; ++j) {
-      issue_tile(j);
+      aim(j);
+      for (int n = 0; n < C::LPW; ++n) part(n);
       __builtin_amdgcn_s_waitcnt(0);
       __syncthreads();
       const uint32_t kb = smem_a + (j & 1) * 2 * C::TBYTES + row_rd;
       const int key0 = wt.tile(j) * kTile + 4 * h;
 #pragma unroll 1
-      for (int t = 0; t < 2 && sight(j); ++t) {
+      for (int t = 0; t < 2 && ((j >= jv0 && j < jv1) || (j == 0 && sinks)); ++t) {
         f32x16 x = zero16(), y = zero16();
 #pragma unroll
         for (int c = 0; c < C::KC; ++c) {
@@ -307,6 +316,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_dq_kernel(WinBwdArgs
       __syncthreads();
     }
     dl = sum_halves(dl);
+    ks = Kg + (size_t)wt.tile(0) * kTile * krs, vs = Vg + (size_t)wt.tile(0) * kTile * vrs;
   }
   if (row_ok && h == 0) {
     a.Dsum[stat] = dl;
@@ -314,23 +324,30 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_dq_kernel(WinBwdArgs
   }
 
   if (wt.n) {
-    issue_tile(0);
+    aim(0);
+    for (int n = 0; n < C::LPW; ++n) part(n);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     int j = 0;
+    // Step j copies tile j + 1 (the last one its own again, to where nothing reads: its parts need no branch)
     auto run = [&](auto tag) __attribute__((always_inline)) {
-      if (j + 1 < wt.n) issue_tile(j + 1);
-      if constexpr (decltype(tag)::value >= 0) tile(j, tag);
+      if (j + 1 < wt.n)
+        aim(j + 1);
+      else
+        dst = smem_a + ((j + 1) & 1) * 2 * C::TBYTES;
+      if constexpr (decltype(tag)::value >= 0)
+        tile(j, tag, part);
+      else
+        for (int n = 0; n < C::LPW; ++n) part(n);
       __builtin_amdgcn_s_waitcnt(0);
       __syncthreads();
       ++j;
     };
-    if (sight(0) && s.sinks > 0)
-      run(IntTag<2>());
+    if (sinks) run(IntTag<2>());
     while (j < wt.n) {
-      while (j < wt.n && sight(j) == 0) run(IntTag<-1>());
-      while (j < wt.n && sight(j) == 1) run(IntTag<1>());
-      while (j < wt.n && sight(j) == 2) run(IntTag<0>());
+      while (j < wt.n && (j < jv0 || j >= jv1)) run(IntTag<-1>());
+      while (j < jv1 && (j < jw0 || j >= jw1)) run(IntTag<1>());
+      while (j < jw1 && j >= jw0 && j < jv1) run(IntTag<0>());
     }
   }
 
@@ -376,15 +393,9 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_dq_kernel(WinBwdArgs
       }
     }
   }
-  if (!row_ok) return;
-#pragma unroll
-  for (int dt = 0; dt < C::DT; ++dt)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const f32x16& o = dQa[dt];
-      *(u32x2*)(dQg + 32 * dt + 8 * g + 4 * h) = u32x2{pack_bf16(o[4 * g] * s.scale, o[4 * g + 1] * s.scale),
-                                                       pack_bf16(o[4 * g + 2] * s.scale, o[4 * g + 3] * s.scale)};
-    }
+  // (every wave is past its last tile)
+  const int rows = i1 - i0 - 32 * wave;
+  store_rows<D>(smem_a + wave * kRowsOut<D>, lane, dQa, s.scale, dQg, s.q_row, [&](int r) { return r <= rows; });
 }
 
 // ---- dK, dV: key owner ----
@@ -417,8 +428,9 @@ struct WinKeyWave {
   //   the d tiles: two products that follow each other never add to the same sum, since the second would
   //   wait for the first to leave the matrix core
   // Beside them p, then dS, of rows 0-31 from slot 2KC, of rows 32-63 from slot 4KC.
-  template <bool MASK>
-  __device__ __forceinline__ void step(uint32_t stage_a, int d0, uint32_t lim) {
+  // part(0 .. NPART): copies of the next rows, issued among the products.
+  template <bool MASK, int NPART, class Part>
+  __device__ __forceinline__ void step(uint32_t stage_a, int d0, uint32_t lim, Part part) {
     constexpr int NS = 4 * C::KC + 8 * C::DT;
     constexpr int PPS = 8 / C::KC;
     uint32_t row_a = stage_a + row_rd, tr_a = stage_a + tr_rd, stat_a = stage_a + C::STAT + st_rd;
@@ -487,6 +499,7 @@ struct WinKeyWave {
     for (int k = 0; k <= ahead(0); ++k) ring[k] = operand(k);
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
+      if ((i & 1) && i / 2 < NPART) part(i / 2);
 #pragma unroll
       for (int k = (i ? i - 1 + ahead(i - 1) : ahead(0)) + 1; k <= i + ahead(i) && k < NS; ++k)
         ring[k % RING] = operand(k);
@@ -594,73 +607,77 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) win_dkdv_kernel(WinBwdAr
       wv.Vr[c] = *(const u32x4*)(vr + 16 * c);
     }
   }
-  uint32_t qoff[C::LPW], goff[C::LPW];
-#pragma unroll
-  for (int n = 0; n < C::LPW; ++n) {
-    qoff[n] = C::copy_offset(wave, lane, n, 0, kTile - 1, qrs);
-    goff[n] = C::copy_offset(wave, lane, n, 0, kTile - 1, grs);
-  }
-  const uint32_t smem_a = lds_at(smem);
-  auto issue_tile = [&](int g, int t, int stage) {
-    const int lo = max(ilo - t * kTile, 0), hi = min(ihi - t * kTile, kTile - 1);
-    const char* qs = Qg + (size_t)t * kTile * qrs + 2 * g * D;
-    const char* gs = Gg + (size_t)t * kTile * grs + 2 * g * D;
-    const uint32_t dst = smem_a + stage * C::STAGE;
-    if (lo == 0 && hi == kTile - 1) {
-#pragma unroll
-      for (int n = 0; n < C::LPW; ++n)
-        if (wave + 4 * n < C::SLOTS) {
-          dma16(qoff[n], qs, dst + 1024 * (wave + 4 * n));
-          dma16(goff[n], gs, dst + C::TBYTES + 1024 * (wave + 4 * n));
-        }
-    } else {
-#pragma unroll
-      for (int n = 0; n < C::LPW; ++n)
-        if (wave + 4 * n < C::SLOTS) {
-          dma16(C::copy_offset(wave, lane, n, lo, hi, qrs), qs, dst + 1024 * (wave + 4 * n));
-          dma16(C::copy_offset(wave, lane, n, lo, hi, grs), gs, dst + C::TBYTES + 1024 * (wave + 4 * n));
-        }
-    }
-    if (wave == 0) {
-      const float* p = a.Dsum + stat0 + (size_t)g * s.TQ + t * kTile + clamp_row(lane, lo, hi);
-      dma4_v(p + stats, dst + C::STAT);
-      dma4_v(p, dst + C::STAT + 256);
-    }
-  };
-  // How tile t sees the wave's 32 keys: not at all (0), in part (1), or every row every key (2; far: the sinks)
-  const int kw0 = k0 + 32 * wave, kw1 = min(kw0 + 31, k1);
-  auto sight = [&](int t) {
-    const int p0 = sq.off + t * kTile, p1 = p0 + kTile - 1;
-    const bool sink = kw0 < s.sinks;
-    if (kw0 > k1 || (far && !sink) || p1 < kw0 || (p0 - kw1 >= s.window && !sink)) return 0;
-    return t * kTile + kTile <= sq.lq && (far || (p0 >= kw1 && p1 - kw0 < s.window)) ? 2 : 1;
-  };
+  // How the tiles of a head see the wave's 32 keys: those of tv0 .. tv1 - 1 at all, of tw0 .. tw1 - 1 whole
+  // (every row every key; far: every sink)
+  const int kw0 = k0 + 32 * wave, kw1 = min(kw0 + 31, k1), tend = tlo + nt;
+  const bool sinks = kw0 < s.sinks;
+  int tv0 = max(tlo, (kw0 - sq.off) >> 6), tv1 = sinks ? tend : min(tend, ((kw0 + 30 + s.window - sq.off) >> 6) + 1);
+  int tw0 = far ? tlo : max(tv0, (kw1 - sq.off + kTile - 1) >> 6);
+  int tw1 = min(far ? tend : ((kw0 + s.window - kTile - sq.off) >> 6) + 1, sq.lq / kTile);
+  if (!wave_on) tv1 = tv0;
+  tw1 = min(tw1, tv1);
+  if (tw0 >= tw1) tw0 = tw1 = tv1;
 
   if (f0 < f1) {
+    const typename C::Slots cp(wave, lane);
+    const uint32_t smem_a = lds_at(smem);
     int f = f0, g = f0 / nt, t = tlo + f0 - g * nt;  // item f: query tile t of head g
-    issue_tile(g, t, 0);
+    // the item to copy: its first rows, and the statistics of tile 0 of its head
+    int tc = t;
+    const char* qs = Qg + (size_t)t * kTile * qrs + 2 * g * D;
+    const char* gs = Gg + (size_t)t * kTile * grs + 2 * g * D;
+    const float* sp = a.Dsum + stat0 + (size_t)g * s.TQ;
+    uint32_t dst = smem_a;
+    auto part = [&](int n) __attribute__((always_inline)) {
+      const int lo = max(ilo - tc * kTile, 0), hi = min(ihi - tc * kTile, kTile - 1);
+      if (n < C::LPW) {
+        cp.copy(n, lo, hi, qs, qrs, gs, grs, dst);
+      } else if (wave == 0) {
+        const float* p = sp + tc * kTile + clamp_row(lane, lo, hi);
+        dma4_v(p + stats, dst + C::STAT);
+        dma4_v(p, dst + C::STAT + 256);
+      }
+    };
+    constexpr int PARTS = C::LPW + 1;
+    for (int n = 0; n < PARTS; ++n) part(n);
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    // the next item is copied while `step` runs on this one
+    // item f + 1 is copied while `step` runs on item f (the last one again, to where nothing reads)
     auto item = [&](auto step) __attribute__((always_inline)) {
-      int gn = g, tn = t + 1;
-      if (tn == tlo + nt) {
-        tn = tlo;
-        ++gn;
+      if (f + 1 < f1) {
+        ++tc;
+        qs += (int64_t)kTile * qrs;
+        gs += (int64_t)kTile * grs;
+        if (tc == tend) {
+          tc = tlo;
+          qs += 2 * D - (int64_t)nt * kTile * qrs;
+          gs += 2 * D - (int64_t)nt * kTile * grs;
+          sp += s.TQ;
+        }
       }
-      if (f + 1 < f1) issue_tile(gn, tn, (f + 1 - f0) & 1);
+      dst = smem_a + ((f + 1 - f0) & 1) * C::STAGE;
       step(smem_a + ((f - f0) & 1) * C::STAGE);
       __builtin_amdgcn_s_waitcnt(0);
       __syncthreads();
-      ++f, g = gn, t = tn;
+      ++f;
+      ++t;
+    };
+    auto idle = [&](uint32_t) {
+      for (int n = 0; n < PARTS; ++n) part(n);
     };
     // loops of one form of the step each (a choice inside one loop costs a copy of the sums per tile); every
     // wave passes every item's barrier
     while (f < f1) {
-      while (f < f1 && sight(t) == 0) item([](uint32_t) {});
-      while (f < f1 && sight(t) == 1)
-        item([&](uint32_t st) { wv.template step<true>(st, sq.off + t * kTile + 4 * h - key, lim); });
-      while (f < f1 && sight(t) == 2) item([&](uint32_t st) { wv.template step<false>(st, 0, 0); });
+      const int te = min(tend, t + f1 - f);  // this head's
+      while (t < te) {
+        while (t < te && (t < tv0 || t >= tv1)) item(idle);
+        while (t < min(te, tv1) && (t < tw0 || t >= tw1))
+          item([&](uint32_t st) {
+            wv.template step<true, PARTS>(st, sq.off + t * kTile + 4 * h - key, lim, part);
+          });
+        while (t < min(te, tw1) && t >= tw0) item([&](uint32_t st) { wv.template step<false, PARTS>(st, 0, 0, part); });
+      }
+      t = tlo;
     }
   }
 
@@ -718,8 +735,13 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) win_dkdv_kernel(WinBwdAr
       }
     }
   }
-  if (key > k1) return;
-  if (split && sink_key) {  // part 0: the block's own rows, then the far parts; fp32 [dK, dV][64][D]
+  const uint32_t lds = lds_at(smem) + wave * kRowsOut<D>;  // (every wave is past its last item)
+  if (!far) {
+    auto live = [&](int r) { return kw0 + r <= k1 && !(split && kw0 + r < s.sinks); };
+    store_rows<D>(lds, lane, wv.st + C::DT, s.scale, a.dK + b * s.k_seq + (size_t)kw0 * s.k_row + kvh * D, s.k_row, live);
+    store_rows<D>(lds, lane, wv.st, 1.0f, a.dV + b * s.v_seq + (size_t)kw0 * s.v_row + kvh * D, s.v_row, live);
+  }
+  if (split && sink_key && key <= k1) {  // part 0: the block's own rows, then the far parts; fp32 [dK, dV][64][D]
     float* out = a.part + ((size_t)group * (a.splits + 1) + (far ? blk + 1 : 0)) * 2 * kWinMaxSinks * D + key * D;
 #pragma unroll
     for (int dt = 0; dt < C::DT; ++dt)
@@ -731,22 +753,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) win_dkdv_kernel(WinBwdAr
         *(f32x4*)(out + d0) = f32x4{k[4 * u], k[4 * u + 1], k[4 * u + 2], k[4 * u + 3]};
         *(f32x4*)(out + kWinMaxSinks * D + d0) = f32x4{v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]};
       }
-    return;
   }
-  if (far) return;
-  uint16_t* dKg = a.dK + b * s.k_seq + (size_t)key * s.k_row + kvh * D;
-  uint16_t* dVg = a.dV + b * s.v_seq + (size_t)key * s.v_row + kvh * D;
-#pragma unroll
-  for (int dt = 0; dt < C::DT; ++dt)
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const f32x16& v = wv.st[dt];
-      const f32x16& k = wv.st[C::DT + dt];
-      const int d0 = 32 * dt + 8 * u + 4 * h;
-      *(u32x2*)(dKg + d0) = u32x2{pack_bf16(k[4 * u] * s.scale, k[4 * u + 1] * s.scale),
-                                  pack_bf16(k[4 * u + 2] * s.scale, k[4 * u + 3] * s.scale)};
-      *(u32x2*)(dVg + d0) = u32x2{pack_bf16(v[4 * u], v[4 * u + 1]), pack_bf16(v[4 * u + 2], v[4 * u + 3])};
-    }
 }
 
 // dK, dV of the sink keys: a workgroup per (sequence, key head) and key; 8 threads to four columns, each with

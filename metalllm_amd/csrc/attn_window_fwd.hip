@@ -74,13 +74,13 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_fwd_kernel(WinFwdArg
   const int i = i0 + 32 * wave + l32;  // this lane's query row
   const bool row_ok = i <= i1;
   const int pos = sq.off + i;
-  uint16_t* Og = a.out + b * s.o_seq + (size_t)min(i, i1) * s.o_row + head * D;
+  uint16_t* Og = a.out + b * s.o_seq + (size_t)(i0 + 32 * wave) * s.o_row + head * D;  // the wave's rows
   float* lg = a.l ? a.l + ((size_t)b * s.NH + head) * s.TQ : nullptr;
 
   if (wt.n == 0) {  // every row stands before the first key
     if (row_ok) {
 #pragma unroll
-      for (int c = 0; c < D / 16; ++c) *(u32x4*)(Og + 16 * c + 8 * h) = u32x4{0, 0, 0, 0};
+      for (int c = 0; c < D / 16; ++c) *(u32x4*)(Og + (size_t)l32 * s.o_row + 16 * c + 8 * h) = u32x4{0, 0, 0, 0};
       if (lg && h == 0) lg[i] = -INFINITY;
     }
     return;
@@ -96,64 +96,53 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_fwd_kernel(WinFwdArg
 #pragma unroll
   for (int c = 0; c < C::KC; ++c) Qr[c] = *(const u32x4*)(Qg + 16 * c + 8 * h);
 
-  // Copies: 1 KB instruction n of a tile covers 16-byte slots 64n .. 64n + 63; slot t is (row t / SLOTS,
-  // chunk t % SLOTS); pad chunks repeat the row's last chunk. Rows of a tile that [lo, hi], the keys that
-  // some row of the workgroup sees, holds in part are held in it.
-  uint32_t koff[C::KPW], voff[C::VPW];  // bytes from the tile's first row
+  // Copies: 1 KB instruction n of the wave covers 16-byte slots 64 (wave + 4n) .. + 63 of a tile; slot t is (row
+  // t / SLOTS, chunk t % SLOTS); pad chunks repeat the row's last one. Rows are held in [lo, hi], the keys
+  // that some row of the workgroup sees. Step j copies V(j) and K(j + 2), in parts that it issues among its
+  // products: issued together before them, addresses and copies took a third of a step.
+  int krow[C::KPW], vrow[C::VPW];
+  uint32_t kchunk[C::KPW], vchunk[C::VPW];
   auto vx = [](int r) { return D == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); };
-  auto slot = [&](int n) { return 64 * (wave + 4 * n) + lane; };
-  auto koff_of = [&](int n, int lo, int hi) {
-    const int t = slot(n), r = t / C::KSLOTS;
-    return __umul24(clamp_row(r, lo, hi), krs) + 16 * min(t - r * C::KSLOTS, D / 8 - 1);
-  };
-  auto voff_of = [&](int n, int lo, int hi) {
-    const int t = slot(n), r = t / C::VSLOTS;
-    return __umul24(clamp_row(r, lo, hi), vrs) + 16 * ((t % C::VSLOTS) ^ vx(r));
-  };
 #pragma unroll
-  for (int n = 0; n < C::KPW; ++n) koff[n] = koff_of(n, 0, C::BN - 1);
+  for (int n = 0; n < C::KPW; ++n) {
+    const int t = 64 * (wave + 4 * n) + lane;
+    krow[n] = t / C::KSLOTS;
+    kchunk[n] = 16 * min(t % C::KSLOTS, D / 8 - 1);
+  }
 #pragma unroll
-  for (int n = 0; n < C::VPW; ++n) voff[n] = voff_of(n, 0, C::BN - 1);
+  for (int n = 0; n < C::VPW; ++n) {
+    const int t = 64 * (wave + 4 * n) + lane;
+    vrow[n] = t / C::VSLOTS;
+    vchunk[n] = 16 * ((t % C::VSLOTS) ^ vx(vrow[n]));
+  }
   const uint32_t smem_a = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char*)smem;
-  // the rows of step j's tile that may be read; whether that is all of them
-  auto rows_of = [&](int j, int kt, int& lo, int& hi) {
-    const bool sink_tile = j < wt.sink;
-    lo = sink_tile ? 0 : max(wt.lo - kt * C::BN, 0);
-    hi = sink_tile ? s.sinks - 1 : min(wt.hi - kt * C::BN, C::BN - 1);
-    return lo == 0 && hi == C::BN - 1;
-  };
-  auto load_k = [&](int j, int stage) {
-    const int kt = wt.tile(j);
+  struct Aim {  // a tile to copy: its first row, the rows to read, the LDS stage
+    const char* src;
     int lo, hi;
-    const bool all = rows_of(j, kt, lo, hi);
-    const char* src = Kg + (size_t)kt * C::BN * krs;
-    const uint32_t dst = smem_a + stage * C::STAGE;
-    if (all) {
-#pragma unroll
-      for (int n = 0; n < C::KPW; ++n)
-        if (wave + 4 * n < C::KSLOTS) dma16(koff[n], src, dst + 1024 * (wave + 4 * n));
-    } else {
-#pragma unroll
-      for (int n = 0; n < C::KPW; ++n)
-        if (wave + 4 * n < C::KSLOTS) dma16(koff_of(n, lo, hi), src, dst + 1024 * (wave + 4 * n));
-    }
+    uint32_t dst;
   };
-  auto load_v = [&](int j, int stage) {
+  auto aim = [&](Aim& x, int j, uint32_t rs, uint32_t dst) {
     const int kt = wt.tile(j);
-    int lo, hi;
-    const bool all = rows_of(j, kt, lo, hi);
-    const char* src = Vg + (size_t)kt * C::BN * vrs;
-    const uint32_t dst = smem_a + stage * C::STAGE + C::KBYTES;
-    if (all) {
-#pragma unroll
-      for (int n = 0; n < C::VPW; ++n)
-        if (wave + 4 * n < C::VSLOTS) dma16(voff[n], src, dst + 1024 * (wave + 4 * n));
-    } else {
-#pragma unroll
-      for (int n = 0; n < C::VPW; ++n)
-        if (wave + 4 * n < C::VSLOTS) dma16(voff_of(n, lo, hi), src, dst + 1024 * (wave + 4 * n));
-    }
+    if (j > 0) x.src += (int64_t)C::BN * (kt - wt.tile(j - 1)) * rs;
+    x.lo = j < wt.sink ? 0 : max(wt.lo - kt * C::BN, 0);
+    x.hi = j < wt.sink ? s.sinks - 1 : min(wt.hi - kt * C::BN, C::BN - 1);
+    x.dst = dst;
   };
+  Aim ka{Kg + (size_t)wt.tile(0) * C::BN * krs, 0, 0, 0}, va{Vg + (size_t)wt.tile(0) * C::BN * vrs, 0, 0, 0};
+  auto copy_k = [&](int n) __attribute__((always_inline)) {
+    if (wave + 4 * n < C::KSLOTS)
+      dma16(__umul24(clamp_row(krow[n], ka.lo, ka.hi), krs) + kchunk[n], ka.src, ka.dst + 1024 * (wave + 4 * n));
+  };
+  auto copy_v = [&](int n) __attribute__((always_inline)) {
+    if (wave + 4 * n < C::VSLOTS)
+      dma16(__umul24(clamp_row(vrow[n], va.lo, va.hi), vrs) + vchunk[n], va.src, va.dst + 1024 * (wave + 4 * n));
+  };
+  constexpr int PARTS = C::KPW + C::VPW;
+  auto part = [&](int n) __attribute__((always_inline)) {
+    if (n < C::VPW) copy_v(n);
+    else copy_k(n - C::VPW);
+  };
+  auto no_part = [](int) {};
 
   // LDS operand bases (elements inside a stage). K rows: A operand of S^T, lane = key row. V^T by
   // transposing reads: group lane/16 covers 16 d of a 32-d tile, source lane t = lane%16 points at key row
@@ -181,7 +170,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_fwd_kernel(WinFwdArg
   // Softmax: slots [0, BSLOT) max of the score pairs, BSLOT the reference point, then exponent,
   // exp2, and sum and packed P in three stages per pair.
   auto wstep = [&](auto flags, int rd, const f32x16& Xc0, const f32x16& Xc1, f32x16& Xn0, f32x16& Xn1,
-                   const uint32_t(&Pin)[16], uint32_t(&Pout)[16]) __attribute__((always_inline)) {
+                   const uint32_t(&Pin)[16], uint32_t(&Pout)[16], auto part) __attribute__((always_inline)) {
     using F = decltype(flags);
     if (F::PV && rescale) {
       asm volatile("" ::: "memory");  // keeps the rescale behind its branch
@@ -219,6 +208,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_fwd_kernel(WinFwdArg
     float t0[16], t1[16], e0[16], e1[16];
 #pragma unroll
     for (int n = 0; n < NV; ++n) {
+      if (n < PARTS) part(n);
       if (n < NM) {
         if (n + RING - 1 < NM) ring[(n + RING - 1) % RING] = operand(n + RING - 1);
         const u32x4& op = ring[n % RING];
@@ -294,9 +284,18 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_fwd_kernel(WinFwdArg
   // Step j: every wave copies K(j + 2) and V(j) into stage j & 1, which the steps before have finished
   // reading, runs its part, then all wait for the copies. Every wave passes every step's barrier.
   const int n = wt.n;
+  auto aim_both = [&](int j) __attribute__((always_inline)) {
+    if (j + 2 < n) {
+      aim(ka, j + 2, krs, smem_a + (j & 1) * C::STAGE);
+    } else {  // the last tile again, to where nothing reads: the parts need no branch
+      ka.dst = smem_a + (j & 1) * C::STAGE;
+    }
+    aim(va, j, vrs, smem_a + (j & 1) * C::STAGE + C::KBYTES);
+  };
   auto copy = [&](int j) __attribute__((always_inline)) {
-    if (j + 2 < n) load_k(j + 2, j & 1);
-    load_v(j, j & 1);
+    aim_both(j);
+#pragma unroll
+    for (int t = 0; t < PARTS; ++t) part(t);
   };
   auto scores = [&](int j) __attribute__((always_inline)) {  // S of tile j into Sc
     const uint16_t* kb = (const uint16_t*)(smem + (j & 1) * C::STAGE) + k_rd;
@@ -345,9 +344,14 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_fwd_kernel(WinFwdArg
   int j = 0;
   auto run = [&](auto flags) __attribute__((always_inline)) {
     using F = decltype(flags);
-    if (j < n) copy(j);
-    if (F::SM) mask(std::bool_constant<!F::PV>(), j, Sc0, Sc1);
-    wstep(flags, (j + 1) & 1, Sc0, Sc1, Sn0, Sn1, Pp, Pc);
+    if (F::SM) {
+      aim_both(j);
+      mask(std::bool_constant<!F::PV>(), j, Sc0, Sc1);
+      wstep(flags, (j + 1) & 1, Sc0, Sc1, Sn0, Sn1, Pp, Pc, part);
+    } else {
+      if (j < n) copy(j);
+      wstep(flags, (j + 1) & 1, Sc0, Sc1, Sn0, Sn1, Pp, Pc, no_part);
+    }
     if (F::S) {
       Sc0 = Sn0;
       Sc1 = Sn1;
@@ -360,8 +364,14 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_fwd_kernel(WinFwdArg
     ++j;
   };
 
-  load_k(0, 0);
-  if (n > 1) load_k(1, 1);
+  aim(ka, 0, krs, smem_a);
+#pragma unroll
+  for (int t = 0; t < C::KPW; ++t) copy_k(t);
+  if (n > 1) {
+    aim(ka, 1, krs, smem_a + C::STAGE);
+#pragma unroll
+    for (int t = 0; t < C::KPW; ++t) copy_k(t);
+  }
   sync();
   if (jw0 == 0) scores(0);
   __syncthreads();
@@ -380,13 +390,13 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_fwd_kernel(WinFwdArg
     run(WfStep<true, false, true>());  // (behind the wave's last tile S is of no use, and unused)
     if (j < jw1 && ((jw1 - j) & 1)) run(WfStep<true, true, true>());
     while (j < jw1) {  // two steps in turn on swapped buffers
-      copy(j);
+      aim_both(j);
       mask(std::false_type(), j, Sc0, Sc1);
-      wstep(WfStep<true, true, true>(), (j + 1) & 1, Sc0, Sc1, Sn0, Sn1, Pp, Pc);
+      wstep(WfStep<true, true, true>(), (j + 1) & 1, Sc0, Sc1, Sn0, Sn1, Pp, Pc, part);
       sync();
-      copy(j + 1);
+      aim_both(j + 1);
       mask(std::false_type(), j + 1, Sn0, Sn1);
-      wstep(WfStep<true, true, true>(), j & 1, Sn0, Sn1, Sc0, Sc1, Pc, Pp);
+      wstep(WfStep<true, true, true>(), j & 1, Sn0, Sn1, Sc0, Sc1, Pc, Pp, part);
       sync();
       j += 2;
     }
@@ -444,20 +454,16 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_fwd_kernel(WinFwdArg
       }
     }
   }
-  if (!row_ok) return;
   const bool empty = pos < 0;
-  const float inv = empty ? 0.0f : 1.0f / lt;
+  const float inv = 1.0f / lt;
 #pragma unroll
   for (int dt = 0; dt < C::DT; ++dt)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      u32x2 w;
-      w[0] = pack_bf16(O[dt][4 * g] * inv, O[dt][4 * g + 1] * inv);
-      w[1] = pack_bf16(O[dt][4 * g + 2] * inv, O[dt][4 * g + 3] * inv);
-      if (empty) w = u32x2{0, 0};
-      *(u32x2*)(Og + 32 * dt + 8 * g + 4 * h) = w;
-    }
-  if (lg && h == 0) lg[i] = empty ? -INFINITY : m_run * s.scale + logf(lt);
+    for (int r = 0; r < 16; ++r) O[dt][r] = empty ? 0.0f : O[dt][r] * inv;
+  if (lg && h == 0 && row_ok) lg[i] = empty ? -INFINITY : m_run * s.scale + logf(lt);
+  __syncthreads();  // every wave is past its last P.V
+  const int rows = i1 - i0 - 32 * wave;
+  store_rows<D>(smem_a + wave * kRowsOut<D>, lane, O, 1.0f, Og, s.o_row, [&](int r) { return r <= rows; });
 }
 
 hipError_t launch_window_forward(const WinFwdArgs& a, int D, hipStream_t s) {
