@@ -10,8 +10,8 @@ from __future__ import annotations
 
 import ctypes
 
-from .attention import _check, _lib, _ptr, _stream
-from .window import on_device
+from .attention import _check, _lib
+from .window import on_device, raw_stream, torch_
 
 MAX_COLS = 8192  # METALLLM_RMSNORM_MAX_COLS
 
@@ -51,32 +51,38 @@ def _shape(t):
 
 
 def _are(dtype, count, *tensors):
+    """The addresses of contiguous tensors (or None) of `count` values."""
+    at = []
     for t in tensors:
-        if t is not None and (t.dtype != dtype or t.numel() != count):
+        if t is None:
+            at.append(None)
+            continue
+        if t.dtype is not dtype or t.numel() != count:
             raise ValueError(f"tensor must hold {count} values of {dtype}")
+        if not t.is_contiguous():
+            raise ValueError("tensor must be contiguous")
+        at.append(t.data_ptr())
+    return at
 
 
 def rmsnormForward(x, residual, sum, out, gamma, rstd=None, eps: float = 1e-5, stream=None):
     """h = x + residual, sum = bf16(h), rstd = 1/sqrt(mean(h^2) + eps), out = bf16(h rstd gamma). residual,
     sum and rstd may be None (a residual needs sum)."""
-    import torch
     rows, cols = _shape(x)
-    on_device(x, residual, sum, out, gamma, rstd)
-    _are(torch.bfloat16, rows * cols, x, residual, sum, out), _are(torch.bfloat16, cols, gamma), _are(torch.float32, rows, rstd)
-    _check(_L().rmsnormForward(_ptr(x), _ptr(residual), _ptr(sum), _ptr(out), _ptr(gamma), _ptr(rstd),
-                               ctypes.byref(RmsnormParams.of(rows, cols, eps)), _stream(stream)), "rmsnormForward")
+    here, T = on_device(x, residual, sum, out, gamma, rstd), torch_()
+    _check(_L().rmsnormForward(*_are(T.bfloat16, rows * cols, x, residual, sum, out), *_are(T.bfloat16, cols, gamma),
+                               *_are(T.float32, rows, rstd), ctypes.byref(RmsnormParams.of(rows, cols, eps)),
+                               raw_stream(stream, here)), "rmsnormForward")
 
 
 def rmsnormForwardFp8(x, residual, sum, out, scales, gamma, rstd=None, eps: float = 1e-5, group: int = 128, stream=None):
     """rmsnormForward with out = e4m3(h rstd gamma / scale), one scale per `group` columns of a row (0: per row)."""
-    import torch
     rows, cols = _shape(x)
-    on_device(x, residual, sum, out, scales, gamma, rstd)
-    _are(torch.bfloat16, rows * cols, x, residual, sum), _are(torch.float8_e4m3fn, rows * cols, out)
-    _are(torch.bfloat16, cols, gamma), _are(torch.float32, rows, rstd)
-    _are(torch.float32, rows * (-(-cols // group) if group > 0 else 1), scales)
-    _check(_L().rmsnormForwardFp8(_ptr(x), _ptr(residual), _ptr(sum), _ptr(out), _ptr(scales), _ptr(gamma), _ptr(rstd),
-                                  ctypes.byref(RmsnormParams.of(rows, cols, eps, group)), _stream(stream)),
+    here, T = on_device(x, residual, sum, out, scales, gamma, rstd), torch_()
+    _check(_L().rmsnormForwardFp8(*_are(T.bfloat16, rows * cols, x, residual, sum), *_are(T.float8_e4m3fn, rows * cols, out),
+                                  *_are(T.float32, rows * (-(-cols // group) if group > 0 else 1), scales),
+                                  *_are(T.bfloat16, cols, gamma), *_are(T.float32, rows, rstd),
+                                  ctypes.byref(RmsnormParams.of(rows, cols, eps, group)), raw_stream(stream, here)),
            "rmsnormForwardFp8")
 
 
@@ -92,12 +98,15 @@ def rmsnormBackward(dOut, dSum, h, gamma, rstd, dX, dgamma, workspace, stream=No
     """dX = dSum + gradient through the norm (the gradient of x and of residual), dgamma written. h is the
     forward's sum; dSum (the residual stream's gradient) may be None; workspace: a tensor of
     backward_workspace_bytes(rows, cols) bytes."""
-    import torch
     rows, cols = _shape(h)
-    on_device(dOut, dSum, h, gamma, rstd, dX, dgamma, workspace)
-    _are(torch.bfloat16, rows * cols, dOut, dSum, h, dX), _are(torch.bfloat16, cols, gamma)
-    _are(torch.float32, rows, rstd), _are(torch.float32, cols, dgamma)
+    here, T = on_device(dOut, dSum, h, gamma, rstd, dX, dgamma, workspace), torch_()
+    at = None
+    if workspace is not None:
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
+        at = workspace.data_ptr()
     n = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    _check(_L().rmsnormBackward(_ptr(dOut), _ptr(dSum), _ptr(h), _ptr(gamma), _ptr(rstd), _ptr(dX), _ptr(dgamma),
-                                _ptr(workspace), n, ctypes.byref(RmsnormParams.of(rows, cols)), _stream(stream)),
-           "rmsnormBackward")
+    dy, ds, hp, dx = _are(T.bfloat16, rows * cols, dOut, dSum, h, dX)
+    _check(_L().rmsnormBackward(dy, ds, hp, *_are(T.bfloat16, cols, gamma), *_are(T.float32, rows, rstd), dx,
+                                *_are(T.float32, cols, dgamma), at, n, ctypes.byref(RmsnormParams.of(rows, cols)),
+                                raw_stream(stream, here)), "rmsnormBackward")

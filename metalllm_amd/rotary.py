@@ -9,8 +9,8 @@ from __future__ import annotations
 
 import ctypes
 
-from .attention import _check, _lib, _stream
-from .window import on_device, row_seq
+from .attention import _check, _lib
+from .window import on_device, raw_stream, row_seq, torch_
 
 PAIRS = 128  # METALLLM_ROTARY_PAIRS
 SCALING = {"none": 0, "linear": 1, "parts": 2}
@@ -65,25 +65,30 @@ def _L():
 
 
 def _rotary(name, q, k, q_out, k_out, positions, plan, stream):
-    import torch
     if (k is None) != (k_out is None):
         raise ValueError("k and k_out go together")
-    on_device(q, k, q_out, k_out, positions)
-    pairs = ((q, q_out),) if k is None else ((q, q_out), (k, k_out))
-    for a, b in pairs:
-        if a.dtype != torch.bfloat16 or b.dtype != torch.bfloat16:
-            raise ValueError("tensors must be bfloat16")
-        if a.dim() != 4 or a.shape != b.shape or a.shape[:2] != q.shape[:2] or a.shape[3] != q.shape[3]:
-            raise ValueError("q, q_out: [B, T, NH, D]; k, k_out: [B, T, NKV, D]")
-    B, T, NH, D = q.shape
-    if positions is not None and (positions.dtype != torch.int32 or positions.shape != (B, T) or not positions.is_contiguous()):
-        raise ValueError("positions must be int32 [B, T], contiguous")
-    none = (0, 0)
-    p = RotaryParams(B, T, NH, 0 if k is None else k.shape[2], D, 0, *row_seq(q), *(none if k is None else row_seq(k)),
-                     *row_seq(q_out), *(none if k is None else row_seq(k_out)))
-    at = lambda t: None if t is None else t.data_ptr()
-    _check(getattr(_L(), name)(q.data_ptr(), at(k), q_out.data_ptr(), at(k_out), at(positions), ctypes.byref(plan),
-                               ctypes.byref(p), _stream(stream)), name)
+    here = on_device(q, k, q_out, k_out, positions)
+    bf16, shape = torch_().bfloat16, q.shape
+    if q.dtype is not bf16 or q_out.dtype is not bf16 or (k is not None and (k.dtype is not bf16 or k_out.dtype is not bf16)):
+        raise ValueError("tensors must be bfloat16")
+    if len(shape) != 4 or q_out.shape != shape:
+        raise ValueError("q, q_out: [B, T, NH, D]")
+    B, T, NH, D = shape
+    NKV, kp, kop, kr, kor = 0, None, None, (0, 0), (0, 0)
+    if k is not None:
+        if k_out.shape != k.shape or len(k.shape) != 4 or k.shape[:2] != shape[:2] or k.shape[3] != D:
+            raise ValueError("k, k_out: [B, T, NKV, D]")
+        NKV, kp, kop, kr, kor = k.shape[2], k.data_ptr(), k_out.data_ptr(), row_seq(k), row_seq(k_out)
+    at = None
+    if positions is not None:
+        if positions.dtype is not torch_().int32 or positions.shape != shape[:2] or not positions.is_contiguous():
+            raise ValueError("positions must be int32 [B, T], contiguous")
+        at = positions.data_ptr()
+    if max(B, T, NH, NKV, D) >= 1 << 32:
+        raise ValueError("sizes are unsigned 32-bit numbers")
+    p = RotaryParams(B, T, NH, NKV, D, 0, *row_seq(q), *kr, *row_seq(q_out), *kor)
+    _check(getattr(_L(), name)(q.data_ptr(), kp, q_out.data_ptr(), kop, at, ctypes.byref(plan), ctypes.byref(p),
+                               raw_stream(stream, here)), name)
 
 
 def rotaryForward(q, k, q_out, k_out, positions, plan: RotaryPlan, stream=None):

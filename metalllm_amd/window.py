@@ -12,7 +12,7 @@ from __future__ import annotations
 
 import ctypes
 
-from .attention import _check, _lib, _stream
+from .attention import _check, _lib
 
 FULL = (1 << 32) - 1  # a window that holds every key
 
@@ -30,23 +30,21 @@ class WindowParams(ctypes.Structure):
             raise ValueError("q, out: [B, TQ, NH, D]; k, v: [B, TK, NKV, D]")
         B, TQ, NH, D = q.shape
         TK, NKV = k.shape[1], k.shape[2]
+        if max(B, TQ, TK, NH, NKV, D) > FULL:
+            raise ValueError("sizes are unsigned 32-bit numbers")
         if k.shape[0] != B or k.shape[3] != D:
             raise ValueError("q and k disagree about B or D")
         window = FULL if window is None else window
         if not 0 <= window <= FULL or not 0 <= sinks <= FULL:
             raise ValueError("window and sinks are unsigned 32-bit numbers")
-        p = cls(B, TQ, TK, NH, NKV, D, window, sinks, *row_seq(q), *row_seq(k), *row_seq(v), *row_seq(out))
-        p.q_is, p.k_is, p.v_is, p.o_is = (_layout(t) for t in (q, k, v, out))
-        return p
-
-
-def _layout(t):
-    return t.shape, t.stride()
+        return cls(B, TQ, TK, NH, NKV, D, window, sinks, *row_seq(q), *row_seq(k), *row_seq(v), *row_seq(out))
 
 
 def row_seq(t):
     """Elements from a token to the next and from a sequence to the next of a [B, T, heads, D] tensor."""
     B, T, H, D = t.shape
+    if t.is_contiguous():
+        return H * D, T * H * D
     s, r, h, e = t.stride()
     if (e != 1 and D > 1) or (h != D and H > 1):
         raise ValueError("a row's heads must lie beside each other (strides ..., D, 1)")
@@ -90,43 +88,55 @@ def backward_workspace_bytes(p: WindowParams) -> int:
     return n.value
 
 
-_CURRENT = None  # torch.cuda.current_device, imported on the first call
+_T = None  # torch, and its current device and raw current stream, from the first call on
+
+
+def torch_():
+    global _T, _device, _raw_stream
+    if _T is None:
+        import torch
+        torch.cuda.init()
+        _T, _device, _raw_stream = torch, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+    return _T
 
 
 def on_device(*tensors):
-    """Raises unless every tensor (or None) lives on the current GPU, which the call launches on."""
-    global _CURRENT
-    if _CURRENT is None:
-        import torch
-        _CURRENT = torch.cuda.current_device
-    for t in tensors:
-        if t is not None and not t.is_cuda:
-            raise ValueError("tensor must live on the GPU")
-    here = _CURRENT()
-    for t in tensors:
-        if t is not None and t.get_device() != here:
-            raise ValueError("tensor must live on the current GPU")
+    """The current GPU, which the call launches on; raises unless every tensor (or None) lives there."""
+    at = {t.get_device() for t in tensors if t is not None}
+    if -1 in at:
+        raise ValueError("tensor must live on the GPU")
+    torch_()
+    here = _device()
+    if at != {here}:
+        raise ValueError("tensor must live on the current GPU")
+    return here
 
 
-def _bf16(layout, *tensors):
-    import torch
+def raw_stream(stream, here: int):
+    """The handle of `stream`, which has to be of the GPU `here`; None: its current stream."""
+    if stream is None:
+        return _raw_stream(here)
+    if getattr(stream, "device_index", here) != here:
+        raise ValueError("stream must be of the current GPU")
+    return stream.cuda_stream
+
+
+def _bf16(shape, row, seq, *tensors):
     for t in tensors:
-        if t.dtype != torch.bfloat16:
+        if t.dtype is not _T.bfloat16:
             raise ValueError("tensor must be bfloat16")
-        if t.shape != layout[0] or t.stride() != layout[1]:
-            raise ValueError(f"tensor must have shape {tuple(layout[0])} and strides {layout[1]}")
+        if t.shape != shape or row_seq(t) != (row, seq):
+            raise ValueError(f"tensor must have shape {shape}, its rows {row} and its sequences {seq} elements apart")
 
 
 def _logsumexp(p, l):
-    import torch
-    if l is not None and (l.dtype != torch.float32 or l.shape != (p.B, p.NH, p.TQ) or not l.is_contiguous()):
+    if l is not None and (l.dtype is not _T.float32 or l.shape != (p.B, p.NH, p.TQ) or not l.is_contiguous()):
         raise ValueError("l must be float32 [B, NH, TQ], contiguous")
 
 
 def _lengths(p, *lengths):
-    import torch
     for t in lengths:
-        if t is not None and (t.dtype != torch.int32 or t.shape != (p.B,) or not t.is_contiguous()):
+        if t is not None and (t.dtype is not _T.int32 or t.shape != (p.B,) or not t.is_contiguous()):
             raise ValueError("lengths must be int32 [B], contiguous")
 
 
@@ -148,12 +158,15 @@ def windowAttentionForward(q, k, v, out, l=None, q_len=None, k_len=None, workspa
     sinks), lengths and workspace (a tensor of forward_workspace_bytes bytes; None where that is 0) as in
     include/metalllm_attn.h."""
     p = params or WindowParams.of(q, k, v, out, window, sinks)
-    on_device(q, k, v, out, l, q_len, k_len, workspace)
-    _bf16(p.q_is, q), _bf16(p.k_is, k), _bf16(p.v_is, v), _bf16(p.o_is, out)
+    here = on_device(q, k, v, out, l, q_len, k_len, workspace)
+    B, D = p.B, p.D
+    rows, keys = (B, p.TQ, p.NH, D), (B, p.TK, p.NKV, D)
+    _bf16(rows, p.q_row, p.q_seq, q), _bf16(keys, p.k_row, p.k_seq, k)
+    _bf16(keys, p.v_row, p.v_seq, v), _bf16(rows, p.o_row, p.o_seq, out)
     _logsumexp(p, l), _lengths(p, q_len, k_len)
     wp, wn = _room(workspace)
     _check(_L().windowAttentionForward(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _address(l),
-                                       _address(q_len), _address(k_len), wp, wn, ctypes.byref(p), _stream(stream)),
+                                       _address(q_len), _address(k_len), wp, wn, ctypes.byref(p), raw_stream(stream, here)),
            "windowAttentionForward")
 
 
@@ -161,13 +174,16 @@ def windowAttentionBackward(dO, O, l, q, k, v, dQ, dK, dV, q_len=None, k_len=Non
                             params: WindowParams | None = None, window: int | None = None, sinks: int = 0):
     """dQ, dK, dV of windowAttentionForward's out = O, l. dO has O's layout, dQ q's, dK k's and dV v's."""
     p = params or WindowParams.of(q, k, v, O, window, sinks)
-    on_device(dO, O, l, q, k, v, dQ, dK, dV, q_len, k_len, workspace)
-    _bf16(p.q_is, q, dQ), _bf16(p.k_is, k, dK), _bf16(p.v_is, v, dV), _bf16(p.o_is, O, dO)
+    here = on_device(dO, O, l, q, k, v, dQ, dK, dV, q_len, k_len, workspace)
+    B, D = p.B, p.D
+    rows, keys = (B, p.TQ, p.NH, D), (B, p.TK, p.NKV, D)
+    _bf16(rows, p.q_row, p.q_seq, q, dQ), _bf16(keys, p.k_row, p.k_seq, k, dK)
+    _bf16(keys, p.v_row, p.v_seq, v, dV), _bf16(rows, p.o_row, p.o_seq, O, dO)
     _logsumexp(p, l), _lengths(p, q_len, k_len)
     wp, wn = _room(workspace)
     _check(_L().windowAttentionBackward(dO.data_ptr(), O.data_ptr(), _address(l), q.data_ptr(), k.data_ptr(),
                                         v.data_ptr(), dQ.data_ptr(), dK.data_ptr(), dV.data_ptr(), _address(q_len),
-                                        _address(k_len), wp, wn, ctypes.byref(p), _stream(stream)),
+                                        _address(k_len), wp, wn, ctypes.byref(p), raw_stream(stream, here)),
            "windowAttentionBackward")
 
 
