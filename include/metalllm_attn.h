@@ -377,8 +377,9 @@ int metalllmSublayerScratch(const AttentionParams* p, uint64_t need[2], uint64_t
  * depend on the params alone. Nothing is allocated and no memset is recorded: every call can be captured.
  * Outputs and workspace must not share memory with inputs (METALLLM_ATTN_E_OVERLAP, judged from a tensor's
  * first element to its last); dQ, dK and dV may be interleaved slices of one buffer.
- * Validation: D in {64, 128}, NH a multiple of NKV, window >= 1, sinks <= 64, TQ, TK <= 2^24, row strides
- * below 2^22, rows and sequences apart from each other, pointers 16-byte aligned (lengths 4). */
+ * Validation: D in {64, 128}, NH a multiple of NKV, window >= 1, sinks <= 64, TQ, TK <= 2^24, B NH < 2^22 and
+ * B NH TQ/128, B NKV (TK/128 + 128) < 2^24, row strides below 2^22, rows and sequences apart from each other,
+ * pointers 16-byte aligned (lengths 4). */
 typedef struct metalllmWindowParams {
   uint32_t B, TQ, TK, NH, NKV, D;
   uint32_t window; /* keys that a row sees up to its own; any value >= TK: all of them */
@@ -460,7 +461,7 @@ int rotaryBackward(const uint16_t* dq, const uint16_t* dk, uint16_t* dq_out, uin
  * fixed order. Its workspace is as window attention's.
  * sum and out (bf16) may each lie in x's or residual's memory, dX in dOut's, dSum's or h's; otherwise
  * outputs are apart from inputs and each other. cols a multiple of 8, at most METALLLM_RMSNORM_MAX_COLS,
- * rows below 2^31, group 0, 32, 64 or 128, pointers 16-byte aligned. Allocates nothing. */
+ * rows below 2^24, group 0, 32, 64 or 128, pointers 16-byte aligned. Allocates nothing. */
 #define METALLLM_RMSNORM_MAX_COLS 8192
 typedef struct metalllmRmsnormParams {
   uint32_t rows, cols;

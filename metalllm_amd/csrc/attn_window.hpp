@@ -131,16 +131,23 @@ inline size_t win_token_floats(const WinShape& s, int D, int splits) {
   return splits > 1 ? (size_t)s.B * s.NKV * tiles * splits * kTokRows * (D + 2) : 0;
 }
 // Parts that the query tiles (of all heads of a group) beyond the windows of the sink keys' block are dealt to
-// (0: there are none), a few tiles each: they run last, in the gaps that the key blocks leave.
-constexpr int kSinkTiles = 4, kSinkSplits = 128;
+// (0: there are none): four tiles each, so that they fill the gaps that the key blocks leave, and no more
+// than the chip can run of them, since each keeps its sums in the workspace.
 inline int win_sink_splits(const WinShape& s) {
   const int64_t far = (int64_t)s.TK - (kBwdBlockN - 1) - s.window;  // rows that see the sinks alone of block 0
   if (s.sinks == 0 || far <= 0) return 0;
-  const int64_t n = (s.G * ((far + kTile - 1) / kTile) + kSinkTiles - 1) / kSinkTiles;
-  return (int)(n < kSinkSplits ? n : kSinkSplits);
+  const int64_t n = (s.G * ((far + kTile - 1) / kTile) + 3) / 4, groups = (int64_t)s.B * s.NKV;
+  const int64_t most = 4096 / groups < 8 ? 8 : 4096 / groups < 128 ? 4096 / groups : 128;
+  return (int)(n < most ? n : most);
 }
-inline size_t win_sink_floats(const WinShape& s, int D, int splits) {
-  return splits ? (size_t)s.B * s.NKV * (splits + 1) * 2 * kWinMaxSinks * D : 0;
+inline size_t win_sink_floats(const WinShape& s, int D, int splits) {  // [group][part][dK, dV][sink][D]
+  return splits ? (size_t)s.B * s.NKV * (splits + 1) * 2 * s.sinks * D : 0;
+}
+// Work items of a launch are counted in 32 bits: whether every grid of a call, in threads, fits.
+inline bool win_grids_fit(const WinShape& s, int D) {
+  const int64_t most = 1ll << 24, heads = (int64_t)s.B * s.NH, groups = (int64_t)s.B * s.NKV;
+  const int64_t qb = (s.TQ + kFwdBlockM - 1) / kFwdBlockM, kb = (s.TK + kBwdBlockN - 1) / kBwdBlockN;
+  return heads < most / 4 && heads * qb < most && groups * (kb + 128) < most && groups * s.sinks * D < most * 64;
 }
 
 hipError_t launch_window_forward(const WinFwdArgs& a, int D, hipStream_t s);

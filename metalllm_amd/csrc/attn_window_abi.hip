@@ -21,21 +21,6 @@ bool strides_ok(const metalllmWindowParams& p, uint64_t T, uint64_t heads, uint6
   return seq >= (T - 1) * row + w || (seq >= w && row >= (p.B - 1) * seq + w);
 }
 
-int validate(const metalllmWindowParams* p) {
-  if (!p) return METALLLM_ATTN_E_NULL;
-  if (p->D != 64 && p->D != 128) return METALLLM_ATTN_E_HEADDIM;
-  if (p->TQ == 0 || p->TK == 0) return METALLLM_ATTN_E_LAYOUT;
-  if (p->B == 0 || p->NH == 0 || p->NKV == 0 || p->NH % p->NKV) return METALLLM_ATTN_E_LAYOUT;
-  if (p->window == 0 || p->sinks > mla::kWinMaxSinks) return METALLLM_ATTN_E_WINDOW;
-  if (p->TQ > kMostRows || p->TK > kMostRows) return METALLLM_ATTN_E_SIZE;
-  const uint64_t blocks = (uint64_t)(p->TQ > p->TK ? p->TQ : p->TK) / 64 + 129;
-  if ((uint64_t)p->B * p->NH > (1u << 24) || (uint64_t)p->B * p->NH * blocks >= (1ull << 31)) return METALLLM_ATTN_E_SIZE;
-  if (!strides_ok(*p, p->TQ, p->NH, p->q_row, p->q_seq) || !strides_ok(*p, p->TK, p->NKV, p->k_row, p->k_seq) ||
-      !strides_ok(*p, p->TK, p->NKV, p->v_row, p->v_seq) || !strides_ok(*p, p->TQ, p->NH, p->o_row, p->o_seq))
-    return METALLLM_ATTN_E_LAYOUT;
-  return METALLLM_ATTN_OK;
-}
-
 mla::WinShape shape_of(const metalllmWindowParams& p, const int32_t* q_len, const int32_t* k_len) {
   mla::WinShape s;
   s.B = (int)p.B, s.TQ = (int)p.TQ, s.TK = (int)p.TK, s.NH = (int)p.NH, s.NKV = (int)p.NKV, s.G = (int)(p.NH / p.NKV);
@@ -46,6 +31,21 @@ mla::WinShape shape_of(const metalllmWindowParams& p, const int32_t* q_len, cons
   s.q_len = q_len, s.k_len = k_len;
   s.scale = 1.0f / std::sqrt((float)p.D);
   return s;
+}
+
+int validate(const metalllmWindowParams* p) {
+  if (!p) return METALLLM_ATTN_E_NULL;
+  if (p->D != 64 && p->D != 128) return METALLLM_ATTN_E_HEADDIM;
+  if (p->TQ == 0 || p->TK == 0) return METALLLM_ATTN_E_LAYOUT;
+  if (p->B == 0 || p->NH == 0 || p->NKV == 0 || p->NH % p->NKV) return METALLLM_ATTN_E_LAYOUT;
+  if (p->window == 0 || p->sinks > mla::kWinMaxSinks) return METALLLM_ATTN_E_WINDOW;
+  if (p->TQ > kMostRows || p->TK > kMostRows) return METALLLM_ATTN_E_SIZE;
+  if ((uint64_t)p->B * p->NH > (1u << 24) || !mla::win_grids_fit(shape_of(*p, nullptr, nullptr), (int)p->D))
+    return METALLLM_ATTN_E_SIZE;
+  if (!strides_ok(*p, p->TQ, p->NH, p->q_row, p->q_seq) || !strides_ok(*p, p->TK, p->NKV, p->k_row, p->k_seq) ||
+      !strides_ok(*p, p->TK, p->NKV, p->v_row, p->v_seq) || !strides_ok(*p, p->TQ, p->NH, p->o_row, p->o_seq))
+    return METALLLM_ATTN_E_LAYOUT;
+  return METALLLM_ATTN_OK;
 }
 
 // the memory from a tensor's first element to its last

@@ -293,7 +293,7 @@ int validate(const metalllmRmsnormParams* p) {
   if (p->rows == 0 || p->cols == 0 || p->cols % 8 || p->cols > METALLLM_RMSNORM_MAX_COLS) return METALLLM_ATTN_E_LAYOUT;
   if (!(p->eps >= 0.0f) || !std::isfinite(p->eps)) return METALLLM_ATTN_E_LAYOUT;
   if (p->group != 0 && p->group != 32 && p->group != 64 && p->group != 128) return METALLLM_ATTN_E_LAYOUT;
-  if (p->rows >= (1u << 31)) return METALLLM_ATTN_E_SIZE;
+  if (p->rows >= (1u << 24)) return METALLLM_ATTN_E_SIZE;  // 256 threads to a row, counted in 32 bits
   return METALLLM_ATTN_OK;
 }
 

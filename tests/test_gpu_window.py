@@ -22,7 +22,8 @@ TOKENS = [
     C(2, 1, 500, 16, 1, 64, 64, 64, [1, 0], [499, 500]), C(2, 1, 300, 6, 2, 128, 1, 0, None, [0, 300]),
     C(1, 1, 5000, 2, 1, 128, 5000, 0), C(1, 1, 5000, 3, 1, 64, 4001, 17), C(2, 3, 400, 4, 2, 64, 100, 4),
     C(2, 5, 260, 8, 2, 128, 70, 3, [5, 2], [260, 4]), C(1, 7, 2500, 8, 1, 64, 1500, 40), C(1, 16, 300, 4, 1, 128, 9, 2),
-    C(2, 4, 3, 2, 2, 64, 2, 1), C(1, 1, 90, 40, 1, 64, 50, 4),
+    C(2, 4, 3, 2, 2, 64, 2, 1), C(1, 1, 90, 40, 1, 64, 50, 4), C(1, 1, 150, 72, 1, 64, 60, 4), C(2, 16, 90, 8, 2, 128, 40, 4),
+    C(1, 17, 90, 2, 2, 64, 40, 4), C(300, 1, 40, 2, 1, 64, 20, 2),
 ]
 ROWS = [
     C(1, 17, 17, 1, 1, 64, 100, 0), C(1, 63, 63, 2, 2, 64, 1, 0), C(1, 64, 64, 2, 1, 128, 64, 0),
