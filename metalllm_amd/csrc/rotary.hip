@@ -4,7 +4,7 @@
 // turns is pos * f_i, reduced to [-1/2, 1/2] in 64 bits (at position 10^6 a 32-bit product would be off by
 // 2^-5 of a turn for the fastest pair) and only then rounded to 32, where v_sin_f32 and v_cos_f32 take
 // turns. A thread owns 8 pairs of a token: it computes their sines once, then turns them in kHeads heads,
-// q and k in one launch. Halves of 8 pairs that are no whole 16-byte chunks go element by element.
+// q and k in one launch.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -38,98 +38,121 @@ __device__ __forceinline__ float hi_f(uint32_t x) { return __uint_as_float(x & 0
 
 constexpr int kHeads = 4;  // heads per thread: the sines of 8 pairs cost about as much as turning two heads
 
-// VEC: R is a multiple of 16, so a chunk's 8 pairs are two 16-byte chunks of the head in either order.
-// Chunks R/16 .. of a head (the part that does not turn) are copied, 16 values each.
-template <bool VEC>
-__global__ void __launch_bounds__(256) rotary_kernel(RotArgs a, int back, uint32_t chunks, uint32_t parts, uint32_t work) {
+struct Place {  // what a thread turns: unit c of heads h0 .. h1 - 1 of a token
+  uint32_t c, token, t, h0, h1;
+  const uint16_t *q, *k;
+  uint16_t *qo, *ko;
+  __device__ __forceinline__ Place(const RotArgs& a, uint32_t id, uint32_t units, uint32_t parts) {
+    const uint32_t rest = id / units;
+    c = id - rest * units;
+    token = rest / parts;
+    h0 = (rest - token * parts) * kHeads;
+    h1 = min(h0 + kHeads, a.p.NH + a.p.NKV);
+    const uint32_t b = token / a.p.T;
+    t = token - b * a.p.T;
+    q = a.q + b * a.p.q_seq + t * a.p.q_row;
+    k = a.k + b * a.p.k_seq + t * a.p.k_row;
+    qo = a.qo + b * a.p.qo_seq + t * a.p.qo_row;
+    ko = a.ko + b * a.p.ko_seq + t * a.p.ko_row;
+  }
+  __device__ __forceinline__ const uint16_t* in(const RotArgs& a, uint32_t h) const {
+    return h < a.p.NH ? q + h * a.p.D : k + (h - a.p.NH) * a.p.D;
+  }
+  __device__ __forceinline__ uint16_t* out(const RotArgs& a, uint32_t h) const {
+    return h < a.p.NH ? qo + h * a.p.D : ko + (h - a.p.NH) * a.p.D;
+  }
+};
+// sine and cosine of pair i at a position, times the magnitude
+__device__ __forceinline__ void turn_of(const RotArgs& a, double pos, uint32_t i, int back, float& cs, float& sn) {
+  double turn = pos * a.plan.turns[i];
+  turn -= rint(turn);
+  const float f = (float)turn;
+  cs = __builtin_amdgcn_cosf(f) * a.plan.magnitude;
+  sn = __builtin_amdgcn_sinf(f) * a.plan.magnitude;
+  if (back) sn = -sn;
+}
+
+// R a multiple of 16: a unit is 8 pairs, two 16-byte chunks of the head in either order; units R/16 .. of a head
+// (the part that does not turn) are copied, 16 values each.
+__global__ void __launch_bounds__(256) rotary_kernel(RotArgs a, int back, uint32_t units, uint32_t parts, uint32_t work) {
   const uint32_t id = blockIdx.x * 256u + threadIdx.x;
   if (id >= work) return;
-  const uint32_t rest = id / chunks, c = id - rest * chunks;
-  const uint32_t token = rest / parts, part = rest - token * parts;
-  const uint32_t b = token / a.p.T, t = token - b * a.p.T;
-  const uint32_t R = a.plan.dims, half = R / 2, turning = (half + 7) / 8;
-  const uint32_t h0 = part * kHeads, h1 = min(h0 + kHeads, a.p.NH + a.p.NKV);
-  const uint16_t* q = a.q + b * a.p.q_seq + t * a.p.q_row;
-  const uint16_t* k = a.k + b * a.p.k_seq + t * a.p.k_row;
-  uint16_t* qo = a.qo + b * a.p.qo_seq + t * a.p.qo_row;
-  uint16_t* ko = a.ko + b * a.p.ko_seq + t * a.p.ko_row;
-
-  const bool copied = c >= turning;  // the part of the head behind the first R: values R + 16 (c - turning) ..
+  const Place w(a, id, units, parts);
+  const uint32_t R = a.plan.dims, half = R / 2, turning = R / 16;
+  const bool copied = w.c >= turning;
   const bool inter = a.plan.interleaved != 0;
-  // VEC: the thread's two 16-byte chunks of a head: values 16c .. 16c + 15 (neighbours paired, or copied) or
-  // 8c .. and half + 8c ..; every load is in flight while the sines are computed
-  const uint32_t d0 = copied ? R + 16 * (c - turning) : inter ? 16 * c : 8 * c;
+  // the chunks: values 16c .. 16c + 15 (neighbours paired, or copied) or 8c .. and half + 8c ..; every load is in
+  // flight while the sines are computed
+  const uint32_t d0 = copied || inter ? 16 * w.c : 8 * w.c;
   const uint32_t d1 = copied || inter ? d0 + 8 : half + d0;
   const bool two = d1 < a.p.D;
   u4 x0[kHeads], x1[kHeads];
-  if (VEC) {
 #pragma unroll
-    for (int n = 0; n < kHeads; ++n) {
-      const uint32_t h = min(h0 + n, h1 - 1);
-      const uint16_t* x = h < a.p.NH ? q + h * a.p.D : k + (h - a.p.NH) * a.p.D;
-      x0[n] = *(const u4*)(x + d0);
-      x1[n] = two ? *(const u4*)(x + d1) : u4{0, 0, 0, 0};
-    }
+  for (int n = 0; n < kHeads; ++n) {
+    const uint16_t* x = w.in(a, min(w.h0 + n, w.h1 - 1));
+    x0[n] = *(const u4*)(x + d0);
+    x1[n] = two ? *(const u4*)(x + d1) : u4{0, 0, 0, 0};
   }
-  const double pos = a.pos ? (double)a.pos[token] : (double)t;
+  const double pos = a.pos ? (double)a.pos[w.token] : (double)w.t;
   float cs[8], sn[8];
 #pragma unroll
-  for (int u = 0; u < 8; ++u) {
-    const uint32_t i = min(8 * c + u, half - 1);
-    double turn = pos * a.plan.turns[i];
-    turn -= rint(turn);
-    const float f = (float)turn;
-    cs[u] = __builtin_amdgcn_cosf(f) * a.plan.magnitude;
-    sn[u] = __builtin_amdgcn_sinf(f) * a.plan.magnitude;
-    if (back) sn[u] = -sn[u];
-  }
-  if (VEC) {
+  for (int u = 0; u < 8; ++u) turn_of(a, pos, min(8 * w.c + u, half - 1), back, cs[u], sn[u]);
 #pragma unroll
-    for (int n = 0; n < kHeads; ++n) {
-      const uint32_t h = h0 + n;
-      if (h >= h1) continue;
-      u4 y0, y1;
-      if (inter) {
+  for (int n = 0; n < kHeads; ++n) {
+    const uint32_t h = w.h0 + n;
+    if (h >= w.h1) continue;
+    u4 y0, y1;
+    if (inter) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float e0 = lo_f(x0[n][w]), o0 = hi_f(x0[n][w]), e1 = lo_f(x1[n][w]), o1 = hi_f(x1[n][w]);
-          y0[w] = pk(e0 * cs[w] - o0 * sn[w], e0 * sn[w] + o0 * cs[w]);
-          y1[w] = pk(e1 * cs[4 + w] - o1 * sn[4 + w], e1 * sn[4 + w] + o1 * cs[4 + w]);
-        }
-      } else {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const float a0 = lo_f(x0[n][w]), a1 = hi_f(x0[n][w]), b0 = lo_f(x1[n][w]), b1 = hi_f(x1[n][w]);
-          y0[w] = pk(a0 * cs[2 * w] - b0 * sn[2 * w], a1 * cs[2 * w + 1] - b1 * sn[2 * w + 1]);
-          y1[w] = pk(a0 * sn[2 * w] + b0 * cs[2 * w], a1 * sn[2 * w + 1] + b1 * cs[2 * w + 1]);
-        }
+      for (int v = 0; v < 4; ++v) {
+        const float e0 = lo_f(x0[n][v]), o0 = hi_f(x0[n][v]), e1 = lo_f(x1[n][v]), o1 = hi_f(x1[n][v]);
+        y0[v] = pk(e0 * cs[v] - o0 * sn[v], e0 * sn[v] + o0 * cs[v]);
+        y1[v] = pk(e1 * cs[4 + v] - o1 * sn[4 + v], e1 * sn[4 + v] + o1 * cs[4 + v]);
       }
-      uint16_t* y = h < a.p.NH ? qo + h * a.p.D : ko + (h - a.p.NH) * a.p.D;
-      *(u4*)(y + d0) = copied ? x0[n] : y0;
-      if (two) *(u4*)(y + d1) = copied ? x1[n] : y1;
-    }
-    return;
-  }
-  if (copied) {
-    for (uint32_t h = h0; h < h1; ++h) {
-      const uint16_t* x = h < a.p.NH ? q + h * a.p.D : k + (h - a.p.NH) * a.p.D;
-      uint16_t* y = h < a.p.NH ? qo + h * a.p.D : ko + (h - a.p.NH) * a.p.D;
-      if (x == y) continue;
-      for (uint32_t d = d0; d < min(d0 + 16, a.p.D); ++d) y[d] = x[d];
-    }
-    return;
-  }
-  for (uint32_t h = h0; h < h1; ++h) {
-    const uint16_t* x = h < a.p.NH ? q + h * a.p.D : k + (h - a.p.NH) * a.p.D;
-    uint16_t* y = h < a.p.NH ? qo + h * a.p.D : ko + (h - a.p.NH) * a.p.D;
+    } else {
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const uint32_t i = 8 * c + u;
-      if (i >= half) break;
-      const uint32_t e = inter ? 2 * i : i, o = inter ? 2 * i + 1 : half + i;
-      const float xe = __uint_as_float((uint32_t)x[e] << 16), xo = __uint_as_float((uint32_t)x[o] << 16);
-      y[e] = (uint16_t)pk(xe * cs[u] - xo * sn[u], 0.0f);
-      y[o] = (uint16_t)pk(xe * sn[u] + xo * cs[u], 0.0f);
+      for (int v = 0; v < 4; ++v) {
+        const float a0 = lo_f(x0[n][v]), a1 = hi_f(x0[n][v]), b0 = lo_f(x1[n][v]), b1 = hi_f(x1[n][v]);
+        y0[v] = pk(a0 * cs[2 * v] - b0 * sn[2 * v], a1 * cs[2 * v + 1] - b1 * sn[2 * v + 1]);
+        y1[v] = pk(a0 * sn[2 * v] + b0 * cs[2 * v], a1 * sn[2 * v + 1] + b1 * cs[2 * v + 1]);
+      }
+    }
+    uint16_t* y = w.out(a, h);
+    *(u4*)(y + d0) = copied ? x0[n] : y0;
+    if (two) *(u4*)(y + d1) = copied ? x1[n] : y1;
+  }
+}
+
+// Any other R: a unit is one pair, or two values of the rest, so that the lanes of a wave read and write
+// beside each other. (8 pairs to a thread, value by value, took 206 us where this takes 53: B = 9, T = 5030, 20
+// heads of 64 with 62 turned, neighbours; halves 190 and 64.)
+template <bool BESIDE>  // the two values of every unit are one 4-byte word
+__global__ void __launch_bounds__(256) rotary_pairs_kernel(RotArgs a, int back, uint32_t units, uint32_t parts, uint32_t work) {
+  const uint32_t id = blockIdx.x * 256u + threadIdx.x;
+  if (id >= work) return;
+  const Place w(a, id, units, parts);
+  const uint32_t half = a.plan.dims / 2;
+  const bool copied = w.c >= half;
+  const uint32_t e = copied || BESIDE ? 2 * w.c : w.c, o = copied ? e + 1 : half + w.c;
+  uint32_t x2[kHeads];
+#pragma unroll
+  for (int n = 0; n < kHeads; ++n) {
+    const uint16_t* x = w.in(a, min(w.h0 + n, w.h1 - 1));
+    x2[n] = BESIDE ? *(const uint32_t*)(x + e) : x[e] | (uint32_t)x[o] << 16;
+  }
+  float cs, sn;
+  turn_of(a, a.pos ? (double)a.pos[w.token] : (double)w.t, min(w.c, half - 1), back, cs, sn);
+#pragma unroll
+  for (int n = 0; n < kHeads; ++n) {
+    if (w.h0 + n >= w.h1) continue;
+    const float a0 = lo_f(x2[n]), b0 = hi_f(x2[n]);
+    const uint32_t y2 = copied ? x2[n] : pk(a0 * cs - b0 * sn, a0 * sn + b0 * cs);
+    uint16_t* y = w.out(a, w.h0 + n);
+    if (BESIDE) {
+      *(uint32_t*)(y + e) = y2;
+    } else {
+      y[e] = (uint16_t)y2;
+      y[o] = (uint16_t)(y2 >> 16);
     }
   }
 }
@@ -160,9 +183,10 @@ int rotary(const uint16_t* q, const uint16_t* k, uint16_t* qo, uint16_t* ko, con
   if (!q || !qo || (p->NKV && (!k || !ko))) return METALLLM_ATTN_E_NULL;
   if (!aligned(q, 16) || !aligned(qo, 16) || !aligned(positions, 4)) return METALLLM_ATTN_E_ALIGN;
   if (p->NKV && (!aligned(k, 16) || !aligned(ko, 16))) return METALLLM_ATTN_E_ALIGN;
-  const uint32_t R = plan->dims, rest = p->D - R;
-  const uint32_t chunks = (R / 2 + 7) / 8 + (rest + 15) / 16, parts = (p->NH + p->NKV + kHeads - 1) / kHeads;
-  const uint64_t work = (uint64_t)p->B * p->T * parts * chunks;
+  const bool whole = plan->dims % 16 == 0;
+  const uint32_t units = whole ? plan->dims / 16 + (p->D - plan->dims + 15) / 16 : p->D / 2;
+  const uint32_t parts = (p->NH + p->NKV + kHeads - 1) / kHeads;
+  const uint64_t work = (uint64_t)p->B * p->T * parts * units;
   if (work >= (1ull << 32) - 256) return METALLLM_ATTN_E_SIZE;
   const dim3 grid((unsigned)((work + 255) / 256));
   // A tensor is turned in place (a thread reads and writes the same values) or into memory of its own;
@@ -179,10 +203,8 @@ int rotary(const uint16_t* q, const uint16_t* k, uint16_t* qo, uint16_t* ko, con
       (positions && mla::any_overlap({sp}, {sqo, sko})))
     return METALLLM_ATTN_E_OVERLAP;
   const RotArgs a{q, k, qo, ko, positions, *p, *plan};
-  if (R % 16 == 0)
-    hipLaunchKernelGGL(rotary_kernel<true>, grid, dim3(256), 0, stream, a, back, chunks, parts, (uint32_t)work);
-  else
-    hipLaunchKernelGGL(rotary_kernel<false>, grid, dim3(256), 0, stream, a, back, chunks, parts, (uint32_t)work);
+  auto* kernel = whole ? rotary_kernel : plan->interleaved ? rotary_pairs_kernel<true> : rotary_pairs_kernel<false>;
+  hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, a, back, units, parts, (uint32_t)work);
   return hipGetLastError() == hipSuccess ? METALLLM_ATTN_OK : METALLLM_ATTN_E_LAUNCH;
 }
 
