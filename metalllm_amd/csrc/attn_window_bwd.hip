@@ -3,7 +3,7 @@
 // With s = q.k/sqrt(D), p = exp(s - l) over the visible keys (l the forward's logsumexp), Dl = sum_d dO.O,
 // dP = dO.v and dS = p (dP - Dl):  dV = P^T.dO,  dK = dS^T.q/sqrt(D),  dQ = dS.k/sqrt(D).
 // Products accumulate in fp32 over all tiles and are rounded once; p and dS are rounded to bf16, the type of
-// the matrix cores' operands (half a step of 2^-8 each, as of the outputs). No atomics: every output has
+// the matrix cores' operands (half a step of 2^-8 each, as of the outputs; FINE: dS in two such parts). No atomics: every output has
 // one owner, and the sum over the query heads of a key head runs in the owner, so results repeat bit for bit.
 //
 // Two kernels, then a small one where there are sinks:
@@ -95,10 +95,22 @@ struct IntTag {
   static constexpr int value = V;
 };
 
+// FINE: a product more with what rounding to bf16 has left of dS, for calls of few rows, over which such errors
+// do not average out: dQ and dK of up to 2176 rows were off by 1.5 times the rounding of the outputs alone, with
+// it by 1.0 times. It takes 22 us instead of 18 at (B, T, NH, NKV, D) = (2, 68, 4, 2, 64), 43 instead of 37 at
+// (1, 1000, 4, 4, 128), both captured; of longer loops it would take a third.
+constexpr int kFineRows = 4096;  // of all heads
+constexpr int kFineItems = 8;    // query tiles of a key block
+// x - bf16(x); 0 where that is no number, so that an infinite x stays one
+__device__ __forceinline__ float rest_bf16(float x) {
+  const float d = x - round_bf16(x);
+  return d - d == 0.0f ? d : 0.0f;
+}
+
 // ---- dQ: query owner ----
 
-template <int D>
-__global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_dq_kernel(WinBwdArgs a) {
+template <int D, bool FINE>
+__global__ void __launch_bounds__(256, FINE ? 1 : D == 64 ? 3 : 2) win_dq_kernel(WinBwdArgs a) {
   using C = WbCfg<D>;
   constexpr int BM = kDqBlockM;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * C::TBYTES];
@@ -204,7 +216,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_dq_kernel(WinBwdArgs
       return (uint32_t)(dq - off) < (uint32_t)s.window || (MASK == 2 && off < sq_);
     };
     f32x16 x0 = zero16(), x1 = zero16(), y0 = zero16(), y1 = zero16();
-    uint32_t dS[16];
+    uint32_t dS[16], low[16];
     constexpr int RING = 6;
     auto ahead = [](int n) { return n < 2 * C::KC || D == 64 ? 5 : 3; };
     u32x4 ring[RING];
@@ -246,6 +258,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_dq_kernel(WinBwdArgs
         uint32_t pk = pack_bf16(d0, d1);
         pin(pk);
         dS[u] = pk;
+        if (FINE) low[u] = pack_bf16(rest_bf16(d0), rest_bf16(d1));
       }
     };
 #pragma unroll
@@ -280,6 +293,12 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : 2) win_dq_kernel(WinBwdArgs
         }
       __builtin_amdgcn_sched_barrier(0);
     }
+    if (FINE)
+#pragma unroll
+      for (int k = 0; k < 4 * C::DT; ++k) {
+        const int dt = k % C::DT, c = k / C::DT;
+        dQa[dt] = mfma(op_of(4 * C::KC + k), u32x4{low[4 * c], low[4 * c + 1], low[4 * c + 2], low[4 * c + 3]}, dQa[dt]);
+      }
   };
 
   // The wave's rows [pw0, pw1] (positions) see tiles of the steps jv0 .. jv1 - 1 (and the sinks in step 0), and
@@ -430,7 +449,8 @@ struct WinKeyWave {
   //   wait for the first to leave the matrix core
   // Beside them p, then dS, of rows 0-31 from slot 2KC, of rows 32-63 from slot 4KC.
   // part(0 .. NPART): copies of the next rows, issued among the products.
-  template <bool MASK, int NPART, class Part>
+  // FINE: with what rounding has left of dS, after the other products.
+  template <bool MASK, bool FINE, int NPART, class Part>
   __device__ __forceinline__ void step(uint32_t stage_a, int d0, uint32_t lim, Part part) {
     constexpr int NS = 4 * C::KC + 8 * C::DT;
     constexpr int PPS = 8 / C::KC;
@@ -440,7 +460,7 @@ struct WinKeyWave {
     pin(stat_a);
     if (MASK) asm volatile("" : "+v"(d0));
     f32x16 x0 = zero16(), x1 = zero16(), y0 = zero16(), y1 = zero16();
-    uint32_t Pp[16], dS[16];
+    uint32_t Pp[16], dS[16], low[16];
     auto operand = [&](int i) -> u32x4 {
       if (i < 4 * C::KC) {
         const int t = i / (2 * C::KC), c = (i % (2 * C::KC)) >> 1;
@@ -487,9 +507,11 @@ struct WinKeyWave {
     };
     auto ds_pair = [&](const f32x16& x, const f32x16& y, int t, int u, float l0, float l1) {
       const int r = 2 * u;
-      uint32_t pk = pack_bf16(x[r] * (y[r] - l0), x[r + 1] * (y[r + 1] - l1));
+      const float d0 = x[r] * (y[r] - l0), d1 = x[r + 1] * (y[r + 1] - l1);
+      uint32_t pk = pack_bf16(d0, d1);
       pin(pk);
       dS[8 * t + u] = pk;
+      if (FINE) low[8 * t + u] = pack_bf16(rest_bf16(d0), rest_bf16(d1));
     };
     constexpr int RING = D == 64 ? 5 : 7;
     constexpr int SA = 3;
@@ -533,11 +555,18 @@ struct WinKeyWave {
       }
       __builtin_amdgcn_sched_barrier(0);
     }
+    if (FINE)
+#pragma unroll
+      for (int k = 0; k < 4 * C::DT; ++k) {
+        const int j = k / C::DT, n = C::DT + k % C::DT;
+        st[n] = mfma(operand(4 * C::KC + 4 * C::DT + k), u32x4{low[4 * j], low[4 * j + 1], low[4 * j + 2], low[4 * j + 3]},
+                     st[n]);
+      }
   }
 };
 
-template <int D>
-__global__ void __launch_bounds__(256, D == 64 ? 2 : 1) win_dkdv_kernel(WinBwdArgs a) {
+template <int D, bool FINE>
+__global__ void __launch_bounds__(256, D == 64 && !FINE ? 2 : 1) win_dkdv_kernel(WinBwdArgs a) {
   using C = WbCfg<D>;
   constexpr int BN = kBwdBlockN;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * C::STAGE];
@@ -674,9 +703,10 @@ __global__ void __launch_bounds__(256, D == 64 ? 2 : 1) win_dkdv_kernel(WinBwdAr
         while (t < te && (t < tv0 || t >= tv1)) item(idle);
         while (t < min(te, tv1) && (t < tw0 || t >= tw1))
           item([&](uint32_t st) {
-            wv.template step<true, PARTS>(st, sq.off + t * kTile + 4 * h - key, lim, part);
+            wv.template step<true, FINE, PARTS>(st, sq.off + t * kTile + 4 * h - key, lim, part);
           });
-        while (t < min(te, tw1) && t >= tw0) item([&](uint32_t st) { wv.template step<false, PARTS>(st, 0, 0, part); });
+        while (t < min(te, tw1) && t >= tw0)
+          item([&](uint32_t st) { wv.template step<false, FINE, PARTS>(st, 0, 0, part); });
       }
       t = tlo;
     }
@@ -784,19 +814,27 @@ __global__ void __launch_bounds__(D * 4) win_sink_kernel(WinBwdArgs a) {
   *(u32x2*)(o + kvh * D + c) = u32x2{pack_bf16(sum[0], sum[1]), pack_bf16(sum[2], sum[3])};
 }
 
-hipError_t launch_window_backward(const WinBwdArgs& a, int D, hipStream_t s) {
+template <int D, bool FINE>
+hipError_t launch(const WinBwdArgs& a, hipStream_t s) {
   const WinShape& p = a.s;
   const unsigned groups = (unsigned)(p.B * p.NKV);
   const unsigned nq = groups * p.G * ((p.TQ + kDqBlockM - 1) / kDqBlockM);
   const unsigned nk = groups * ((p.TK + kBwdBlockN - 1) / kBwdBlockN + a.splits);
-  hipLaunchKernelGGL((D == 64 ? win_dq_kernel<64> : win_dq_kernel<128>), dim3(nq), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((win_dq_kernel<D, FINE>), dim3(nq), dim3(256), 0, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((D == 64 ? win_dkdv_kernel<64> : win_dkdv_kernel<128>), dim3(nk), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((win_dkdv_kernel<D, FINE>), dim3(nk), dim3(256), 0, s, a);
   e = hipGetLastError();
   if (e != hipSuccess || a.splits == 0) return e;
-  hipLaunchKernelGGL((D == 64 ? win_sink_kernel<64> : win_sink_kernel<128>), dim3(groups * p.sinks), dim3(D * 4), 0, s, a);
+  hipLaunchKernelGGL(win_sink_kernel<D>, dim3(groups * p.sinks), dim3(D * 4), 0, s, a);
   return hipGetLastError();
+}
+
+hipError_t launch_window_backward(const WinBwdArgs& a, int D, hipStream_t s) {
+  const WinShape& p = a.s;
+  const bool fine = (int64_t)p.B * p.NH * p.TQ <= kFineRows && p.G * ((p.TQ + kTile - 1) / kTile) <= kFineItems;
+  if (D == 64) return fine ? launch<64, true>(a, s) : launch<64, false>(a, s);
+  return fine ? launch<128, true>(a, s) : launch<128, false>(a, s);
 }
 
 }  // namespace mla

@@ -87,6 +87,22 @@ def check(c, d, got, want=None):
         assert np.isnan(rest).all(), f"{n}: rows behind the lengths were written"
 
 
+def crowd(c, d, want):
+    """The case again with its sequences repeated to more than 4096 rows in all: a backward pass over fewer takes
+    dS in two parts of bf16."""
+    n = 4096 // (c["B"] * c["NH"] * c["TQ"]) + 1
+    c = dict(c, B=c["B"] * n, **{m: c[m] and c[m] * n for m in ("q_len", "k_len")})
+    d = {m: x if x is None else x.repeat(n, *[1] * (x.ndim - 1)) for m, x in d.items()}
+    return c, d, {m: tuple(np.concatenate([x] * n) for x in w) for m, w in want.items()}
+
+
+def check_twice(c, d, gpu, want=None, **k):
+    want = want or reference(c, d)
+    check(c, d, run(c, d, gpu, **k), want)
+    c, d, want = crowd(c, d, want)
+    check(c, d, run(c, d, gpu, **k), want)
+
+
 @pytest.mark.parametrize("c", TOKENS, ids=name_of)
 def test_tokens(gpu, c):
     d = make(c)
@@ -96,13 +112,13 @@ def test_tokens(gpu, c):
 @pytest.mark.parametrize("c", ROWS, ids=name_of)
 def test_rows(gpu, c):
     d = make(c)
-    check(c, d, run(c, d, gpu))
+    check_twice(c, d, gpu)
 
 
 @pytest.mark.parametrize("c", [TOKENS[5], TOKENS[11]], ids=name_of)
 def test_gradient_of_few_rows(gpu, c):
     d = make(c)
-    check(c, d, run(c, d, gpu))
+    check_twice(c, d, gpu)
 
 
 @pytest.mark.parametrize("layout", ["packed", "token first"])
@@ -141,6 +157,8 @@ def test_hidden_values_are_not_read(gpu, c):
             first = max(0, lk - lq - c["window"] + 1)
             assert (got[n][b, min(c["sinks"], first):first] == 0).all()
     check(c, d, got, want)
+    c, d, want = crowd(c, d, want)
+    check(c, d, run(c, d, gpu), want)
 
 
 @pytest.mark.parametrize("where", ["k", "v", "q", "dO"])
@@ -151,7 +169,7 @@ def test_values_that_are_not_finite_reach_their_rows_alone(gpu, c, where):
     d[where][0, at, 0, 5] = float("nan")
     if where == "v":
         d[where][0, at + 4, 0, 9] = float("inf")
-    check(c, d, run(c, d, gpu))
+    check_twice(c, d, gpu)
 
 
 def test_results_repeat(gpu):
