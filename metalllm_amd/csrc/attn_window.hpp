@@ -83,7 +83,6 @@ __device__ __forceinline__ WinTiles win_tiles(const WinShape& s, const WinSeq& q
   return w;
 }
 
-// Rows of one head as the query side of a workgroup or the key side of another see them.
 __device__ __forceinline__ int clamp_row(int r, int lo, int hi) { return min(max(r, lo), hi); }
 
 // A wave's 32 rows x D outputs, held as accumulators (lane: row l32, values 32 dt + 8g + 4h + 0..3 in registers
@@ -131,12 +130,12 @@ inline size_t win_token_floats(const WinShape& s, int D, int splits) {
   return splits > 1 ? (size_t)s.B * s.NKV * tiles * splits * kTokRows * (D + 2) : 0;
 }
 // Parts that the query tiles (of all heads of a group) beyond the windows of the sink keys' block are dealt to
-// (0: there are none): four tiles each, so that they fill the gaps that the key blocks leave, and no more
-// than the chip can run of them, since each keeps its sums in the workspace.
+// (0: there are none): two tiles for each wave of a workgroup, so that they fill the gaps that the key blocks
+// leave, and no more than the chip can run of them, since each keeps its sums in the workspace.
 inline int win_sink_splits(const WinShape& s) {
   const int64_t far = (int64_t)s.TK - (kBwdBlockN - 1) - s.window;  // rows that see the sinks alone of block 0
   if (s.sinks == 0 || far <= 0) return 0;
-  const int64_t n = (s.G * ((far + kTile - 1) / kTile) + 3) / 4, groups = (int64_t)s.B * s.NKV;
+  const int64_t n = (s.G * ((far + kTile - 1) / kTile) + 7) / 8, groups = (int64_t)s.B * s.NKV;
   const int64_t most = 4096 / groups < 8 ? 8 : 4096 / groups < 128 ? 4096 / groups : 128;
   return (int)(n < most ? n : most);
 }

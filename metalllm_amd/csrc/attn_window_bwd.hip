@@ -569,7 +569,7 @@ template <int D, bool FINE>
 __global__ void __launch_bounds__(256, D == 64 && !FINE ? 2 : 1) win_dkdv_kernel(WinBwdArgs a) {
   using C = WbCfg<D>;
   constexpr int BN = kBwdBlockN;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * C::STAGE];
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * C::STAGE];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, l32 = lane & 31;
@@ -614,11 +614,14 @@ __global__ void __launch_bounds__(256, D == 64 && !FINE ? 2 : 1) win_dkdv_kernel
   const int f0 = far ? (int)((int64_t)items * blk / a.splits) : 0;
   const int f1 = far ? (int)((int64_t)items * (blk + 1) / a.splits) : items;
 
-  const int key = k0 + 32 * wave + l32;
+  // far: a wave takes every fs-th item alone, for 32 sinks
+  const int halves = far ? (s.sinks + 31) / 32 : 1, fs = far ? 4 / halves : 1, fw = far ? f0 + wave / halves : f0;
+  const int kw0 = far ? 32 * (wave % halves) : k0 + 32 * wave, kw1 = min(kw0 + 31, k1);
+  const int key = kw0 + l32;
   const bool sink_key = key < s.sinks;
   const int most = sq.lk - key;  // rows of the sequence that stand at the key or behind it
   const uint32_t lim = (uint32_t)max(0, sink_key ? most : far ? 0 : min(s.window, most));
-  const bool wave_on = far ? 32 * wave < s.sinks : k0 + 32 * wave <= k1;
+  const bool wave_on = kw0 <= k1;
 
   const char* Qg = (const char*)(a.q + b * s.q_seq + kvh * s.G * D);
   const char* Gg = (const char*)(a.dO + b * s.o_seq + kvh * s.G * D);
@@ -638,17 +641,39 @@ __global__ void __launch_bounds__(256, D == 64 && !FINE ? 2 : 1) win_dkdv_kernel
     }
   }
   // How the tiles of a head see the wave's 32 keys: those of tv0 .. tv1 - 1 at all, of tw0 .. tw1 - 1 whole
-  // (every row every key; far: every sink)
-  const int kw0 = k0 + 32 * wave, kw1 = min(kw0 + 31, k1), tend = tlo + nt;
+  // (every row every key)
+  const int tend = tlo + nt;
   const bool sinks = kw0 < s.sinks;
   int tv0 = max(tlo, (kw0 - sq.off) >> 6), tv1 = sinks ? tend : min(tend, ((kw0 + 30 + s.window - sq.off) >> 6) + 1);
-  int tw0 = far ? tlo : max(tv0, (kw1 - sq.off + kTile - 1) >> 6);
-  int tw1 = min(far ? tend : ((kw0 + s.window - kTile - sq.off) >> 6) + 1, sq.lq / kTile);
+  int tw0 = max(tv0, (kw1 - sq.off + kTile - 1) >> 6);
+  int tw1 = min(((kw0 + s.window - kTile - sq.off) >> 6) + 1, sq.lq / kTile);
   if (!wave_on) tv1 = tv0;
   tw1 = min(tw1, tv1);
   if (tw0 >= tw1) tw0 = tw1 = tv1;
 
-  if (f0 < f1) {
+  if (far) {
+    const uint32_t st = lds_at(smem) + wave * C::STAGE;
+    for (int f = fw; f < f1; f += fs) {
+      const int g = f / nt, t = tlo + f - g * nt;
+      const int lo = max(ilo - t * kTile, 0), hi = min(ihi - t * kTile, kTile - 1);
+      const char* qs = Qg + (size_t)t * kTile * qrs + 2 * g * D;
+      const char* gs = Gg + (size_t)t * kTile * grs + 2 * g * D;
+      const float* sp = a.Dsum + stat0 + (size_t)g * s.TQ + t * kTile + clamp_row(lane, lo, hi);
+#pragma unroll 1
+      for (int w = 0; w < 4; ++w) {
+        const typename C::Slots cp(w, lane);
+#pragma unroll
+        for (int n = 0; n < C::LPW; ++n) cp.copy(n, lo, hi, qs, qrs, gs, grs, st);
+      }
+      dma4_v(sp + stats, st + C::STAT);
+      dma4_v(sp, st + C::STAT + 256);
+      __builtin_amdgcn_s_waitcnt(0);
+      asm volatile("" ::: "memory");
+      wv.template step<true, FINE, 0>(st, sq.off + t * kTile + 4 * h - key, lim, [](int) {});
+      __builtin_amdgcn_s_waitcnt(0);
+      asm volatile("" ::: "memory");
+    }
+  } else if (f0 < f1) {
     const typename C::Slots cp(wave, lane);
     const uint32_t smem_a = lds_at(smem);
     int f = f0, g = f0 / nt, t = tlo + f0 - g * nt;  // item f: query tile t of head g
@@ -712,7 +737,7 @@ __global__ void __launch_bounds__(256, D == 64 && !FINE ? 2 : 1) win_dkdv_kernel
     }
   }
 
-  if (!wave_on) return;
+  if (!wave_on && !far) return;
   // A row that does not see a key but shares its tile adds 0 * NaN to it where q or dO is not finite: such
   // keys are summed again over the rows that see them.
   float bad = 0.0f;
@@ -726,7 +751,7 @@ __global__ void __launch_bounds__(256, D == 64 && !FINE ? 2 : 1) win_dkdv_kernel
 #pragma unroll
       for (int n = 0; n < 2 * C::DT; ++n) wv.st[n] = zero16();
       bool lost = false;  // p is not a number: then no sum of the key is
-      for (int f = f0; f < f1 && !lost; ++f) {
+      for (int f = fw; f < f1 && !lost; f += fs) {
         const int g = f / nt, t = tlo + f - g * nt;
         const int ra = max(ilo, t * kTile), rb = min(ihi, t * kTile + kTile - 1);
         for (int i = ra; i <= rb && !lost; ++i) {
@@ -774,8 +799,14 @@ __global__ void __launch_bounds__(256, D == 64 && !FINE ? 2 : 1) win_dkdv_kernel
     store_rows<D>(lds, lane, wv.st + C::DT, s.scale, a.dK + b * s.k_seq + (size_t)kw0 * s.k_row + kvh * D, s.k_row, live);
     store_rows<D>(lds, lane, wv.st, 1.0f, a.dV + b * s.v_seq + (size_t)kw0 * s.v_row + kvh * D, s.v_row, live);
   }
-  if (split && sink_key && key <= k1) {  // part 0: the block's own rows, then the far parts; fp32 [dK, dV][sink][D]
-    float* out = a.part + ((size_t)group * (a.splits + 1) + (far ? blk + 1 : 0)) * 2 * s.sinks * D + key * D;
+  if (!split) return;
+  // sums of the sinks, fp32 [dK, dV][sink][D]: part 0 the block's own rows, then the far parts, whose waves
+  // join theirs in LDS
+  float* out = a.part + ((size_t)group * (a.splits + 1) + (far ? blk + 1 : 0)) * 2 * s.sinks * D;
+  float* own = (float*)(smem + wave * C::STAGE);
+  float *ko = far ? own + l32 * 2 * D : out + key * D, *vo = far ? ko + D : ko + s.sinks * D;
+  static_assert(32 * 2 * D * 4 <= C::STAGE, "a wave's sums in its stage");
+  if (sink_key && key <= k1)
 #pragma unroll
     for (int dt = 0; dt < C::DT; ++dt)
 #pragma unroll
@@ -783,9 +814,16 @@ __global__ void __launch_bounds__(256, D == 64 && !FINE ? 2 : 1) win_dkdv_kernel
         const f32x16& v = wv.st[dt];
         const f32x16& k = wv.st[C::DT + dt];
         const int d0 = 32 * dt + 8 * u + 4 * h;
-        *(f32x4*)(out + d0) = f32x4{k[4 * u], k[4 * u + 1], k[4 * u + 2], k[4 * u + 3]};
-        *(f32x4*)(out + s.sinks * D + d0) = f32x4{v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]};
+        *(f32x4*)(ko + d0) = f32x4{k[4 * u], k[4 * u + 1], k[4 * u + 2], k[4 * u + 3]};
+        *(f32x4*)(vo + d0) = f32x4{v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]};
       }
+  if (!far) return;
+  __syncthreads();
+  for (int n = tid; n < min(s.sinks, sq.lk) * (D / 2); n += 256) {
+    const int j = n / (D / 2), c = 4 * (n % (D / 2));
+    f32x4 sum = {0, 0, 0, 0};
+    for (int w = j / 32; w < 4; w += halves) sum += *(const f32x4*)(smem + w * C::STAGE + 4 * ((j & 31) * 2 * D + c));
+    *(f32x4*)(out + (c < D ? j * D + c : (s.sinks + j) * D + c - D)) = sum;
   }
 }
 
