@@ -46,7 +46,7 @@ struct WinBwdArgs {
   uint16_t* dK;
   uint16_t* dV;
   WinShape s;
-  float* Dsum;  // [B, NH, TQ] workspace: sum over d of dO * O
+  float* Dsum;  // [B, NH, TQ] workspace, twice: -Dl (Dl = sum over d of dO O), l log2(e)
   float* part;  // workspace: partial dK, dV of the sink keys, or NULL where nothing is split (splits = 0)
   int splits;
 };

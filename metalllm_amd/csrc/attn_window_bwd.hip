@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(256, FINE ? 1 : D == 64 ? 3 : 2) win_dq_kernel
     ks = Kg + (size_t)wt.tile(0) * kTile * krs, vs = Vg + (size_t)wt.tile(0) * kTile * vrs;
   }
   if (row_ok && h == 0) {
-    a.Dsum[stat] = dl;
+    a.Dsum[stat] = -dl;
     a.Dsum[stats + stat] = l2;
   }
 
@@ -425,9 +425,15 @@ __global__ void __launch_bounds__(256, FINE ? 1 : D == 64 ? 3 : 2) win_dq_kernel
 template <int D>
 struct WinKeyWave {
   using C = WbCfg<D>;
+  static constexpr int NS = 4 * C::KC + 8 * C::DT;  // slots of a step
+  static constexpr bool PRIME = D == 128;           // a step's last slots read the next one's first operands
+  static constexpr int RING = PRIME ? 8 : 5;
+  static_assert(!PRIME || NS % RING == 0, "an operand keeps its place in the ring");
   int h;
   float sl;
   uint32_t row_rd, tr_rd, st_rd;
+  u32x4 ring[RING];  // operands, RING - 1 slots ahead
+  f32x16 first;      // -Dl of rows 0-31 of the next step
   u32x4 Kr[C::KC], Vr[C::KC];
   f32x16 st[2 * C::DT];
 
@@ -442,6 +448,26 @@ struct WinKeyWave {
     for (int n = 0; n < 2 * C::DT; ++n) st[n] = zero16();
   }
 
+  // S and dP operand i of the rows staged at stage_a (+ row_rd)
+  __device__ __forceinline__ u32x4 row_operand(uint32_t row_a, int i) const {
+    const int t = i / (2 * C::KC), c = (i % (2 * C::KC)) >> 1;
+    return lds_b128_w(row_a + ((i & 1) ? C::TBYTES : 0) + 2 * (32 * t * C::P + 16 * c));
+  }
+  // -Dl of rows 32t .. 32t + 31 where the accumulators of dP have them
+  __device__ __forceinline__ void minus_dl(f32x16& y, uint32_t stat_a, int t) const {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 v = lds_f4_w(stat_a + 256 + 4 * (32 * t + 8 * g));
+#pragma unroll
+      for (int r = 0; r < 4; ++r) y[4 * g + r] = v[r];
+    }
+  }
+  __device__ __forceinline__ void prime(uint32_t stage_a) {
+#pragma unroll
+    for (int k = 0; k < RING - 1; ++k) ring[k] = row_operand(stage_a + row_rd, k);
+    minus_dl(first, stage_a + C::STAT + st_rd, 0);
+  }
+
   // Query rows staged at LDS byte address stage_a; MASK: row r of the tile (position p0 + r) sees the lane's
   // key where (uint)(p0 + r - key) < lim; d0 = p0 + 4h - key. Slots (one product each):
   //   [0, 2KC) S and dP of rows 0-31 in turn, [2KC, 4KC) of rows 32-63, then dV and dK, 16 rows at a time over
@@ -451,21 +477,24 @@ struct WinKeyWave {
   // part(0 .. NPART): copies of the next rows, issued among the products.
   // FINE: with what rounding has left of dS, after the other products.
   template <bool MASK, bool FINE, int NPART, class Part>
-  __device__ __forceinline__ void step(uint32_t stage_a, int d0, uint32_t lim, Part part) {
-    constexpr int NS = 4 * C::KC + 8 * C::DT;
+  __device__ __forceinline__ void step(uint32_t stage_a, uint32_t next_a, int d0, uint32_t lim, Part part) {
     constexpr int PPS = 8 / C::KC;
     uint32_t row_a = stage_a + row_rd, tr_a = stage_a + tr_rd, stat_a = stage_a + C::STAT + st_rd;
+    uint32_t next_row_a = next_a + row_rd, next_stat_a = next_a + C::STAT + st_rd;
     pin(row_a);
     pin(tr_a);
     pin(stat_a);
+    if (PRIME) {
+      pin(next_row_a);
+      pin(next_stat_a);
+    }
     if (MASK) asm volatile("" : "+v"(d0));
-    f32x16 x0 = zero16(), x1 = zero16(), y0 = zero16(), y1 = zero16();
+    if (!PRIME) prime(stage_a);
+    f32x16 x0 = zero16(), x1 = zero16(), y0 = first, y1;  // y: dP - Dl
     uint32_t Pp[16], dS[16], low[16];
     auto operand = [&](int i) -> u32x4 {
-      if (i < 4 * C::KC) {
-        const int t = i / (2 * C::KC), c = (i % (2 * C::KC)) >> 1;
-        return lds_b128_w(row_a + ((i & 1) ? C::TBYTES : 0) + 2 * (32 * t * C::P + 16 * c));
-      }
+      if (i >= NS) return row_operand(next_row_a, i - NS);
+      if (i < 4 * C::KC) return row_operand(row_a, i);
       const int k = i - 4 * C::KC, j = k / C::DT % 4, dt = k % C::DT;
       const uint32_t src = tr_a + (k >= 4 * C::DT ? 0 : C::TBYTES) + 2 * (16 * j * C::P + 32 * dt);
       const u32x2 lo = lds_tr_w(src), hi = lds_tr_w(src + 2 * 8 * C::P);
@@ -481,13 +510,8 @@ struct WinKeyWave {
       return n < 8 ? Work{1, t, n, PPS} : Work{2, t, n - 8, PPS};
     };
     static_assert(C::KC == 2 * C::DT, "slots of a half's vector work");
-    auto stats = [&](int i) -> f32x4 {
-      const Work w = work(i);
-      const uint32_t ad = stat_a + (w.kind == 2 ? 256 : 0) + 4 * (32 * w.t + 8 * (w.u0 >> 1) + 2 * (w.u0 & 1));
-      if (w.cnt == 2) return lds_f4_w(ad);
-      const f32x2 v = *(const __attribute__((address_space(3))) f32x2*)(uintptr_t)ad;
-      return f32x4{v[0], v[1], 0.0f, 0.0f};
-    };
+    // l log2(e) of pairs u and u + 1 (u even) of half t
+    auto stats = [&](int t, int u) { return lds_f4_w(stat_a + 4 * (32 * t + 4 * u)); };
     auto seen = [&](int t, int r) { return (uint32_t)(d0 + 32 * t + 8 * (r >> 2) + (r & 3)) < lim; };
     auto p_pair = [&](f32x16& x, int t, int u, float l0, float l1) {
       const int r = 2 * u;
@@ -505,28 +529,23 @@ struct WinKeyWave {
       pin(pk);
       Pp[8 * t + u] = pk;
     };
-    auto ds_pair = [&](const f32x16& x, const f32x16& y, int t, int u, float l0, float l1) {
+    auto ds_pair = [&](const f32x16& x, const f32x16& y, int t, int u) {
       const int r = 2 * u;
-      const float d0 = x[r] * (y[r] - l0), d1 = x[r + 1] * (y[r + 1] - l1);
+      const float d0 = x[r] * y[r], d1 = x[r + 1] * y[r + 1];
       uint32_t pk = pack_bf16(d0, d1);
       pin(pk);
       dS[8 * t + u] = pk;
       if (FINE) low[8 * t + u] = pack_bf16(rest_bf16(d0), rest_bf16(d1));
     };
-    constexpr int RING = D == 64 ? 5 : 7;
     constexpr int SA = 3;
-    auto ahead = [](int) { return RING - 1; };
-    u32x4 ring[RING];
-    f32x4 sring[SA + 1];
-#pragma unroll
-    for (int k = 0; k <= ahead(0); ++k) ring[k] = operand(k);
+    f32x4 sring[4];
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
       if ((i & 1) && i / 2 < NPART) part(i / 2);
-#pragma unroll
-      for (int k = (i ? i - 1 + ahead(i - 1) : ahead(0)) + 1; k <= i + ahead(i) && k < NS; ++k)
-        ring[k % RING] = operand(k);
-      if (i + SA < NS && work(i + SA).kind) sring[(i + SA) % (SA + 1)] = stats(i + SA);
+      if (PRIME || i + RING - 1 < NS) ring[(i + RING - 1) % RING] = operand(i + RING - 1);
+      if (const Work w = work(i + SA); w.kind == 1 && w.u0 % 2 == 0) sring[w.u0 / 2] = stats(w.t, w.u0);
+      if (i == C::KC) minus_dl(y1, stat_a, 1);
+      if (PRIME && i == NS - RING) minus_dl(first, next_stat_a, 0);
       const u32x4& op = ring[i % RING];
       if (i < 4 * C::KC) {
         const int t = i / (2 * C::KC), c = (i % (2 * C::KC)) >> 1;
@@ -544,13 +563,12 @@ struct WinKeyWave {
       }
       const Work w = work(i);
       if (w.cnt) {
-        const f32x4 sv = sring[i % (SA + 1)];
 #pragma unroll
-        for (int v = 0; v < w.cnt; ++v) {
+        for (int u = w.u0; u < w.u0 + w.cnt; ++u) {
           if (w.kind == 1)
-            p_pair(w.t ? x1 : x0, w.t, w.u0 + v, sv[2 * v], sv[2 * v + 1]);
+            p_pair(w.t ? x1 : x0, w.t, u, sring[u / 2][2 * (u % 2)], sring[u / 2][2 * (u % 2) + 1]);
           else
-            ds_pair(w.t ? x1 : x0, w.t ? y1 : y0, w.t, w.u0 + v, sv[2 * v], sv[2 * v + 1]);
+            ds_pair(w.t ? x1 : x0, w.t ? y1 : y0, w.t, u);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -669,20 +687,22 @@ __global__ void __launch_bounds__(256, D == 64 && !FINE ? 2 : 1) win_dkdv_kernel
       dma4_v(sp, st + C::STAT + 256);
       __builtin_amdgcn_s_waitcnt(0);
       asm volatile("" ::: "memory");
-      wv.template step<true, FINE, 0>(st, sq.off + t * kTile + 4 * h - key, lim, [](int) {});
+      if (wv.PRIME) wv.prime(st);
+      wv.template step<true, FINE, 0>(st, st, sq.off + t * kTile + 4 * h - key, lim, [](int) {});
       __builtin_amdgcn_s_waitcnt(0);
       asm volatile("" ::: "memory");
     }
   } else if (f0 < f1) {
     const typename C::Slots cp(wave, lane);
-    const uint32_t smem_a = lds_at(smem);
     int f = f0, g = f0 / nt, t = tlo + f0 - g * nt;  // item f: query tile t of head g
     // the item to copy: its first rows, and the statistics of tile 0 of its head
-    int tc = t;
+    int fc = f, tc = t;
     const char* qs = Qg + (size_t)t * kTile * qrs + 2 * g * D;
     const char* gs = Gg + (size_t)t * kTile * grs + 2 * g * D;
     const float* sp = a.Dsum + stat0 + (size_t)g * s.TQ;
-    uint32_t dst = smem_a;
+    // stages of item f, of those behind it, and of the item to copy
+    constexpr int AHEAD = wv.PRIME ? 2 : 1;
+    uint32_t st = lds_at(smem), next = st + C::STAGE, dst = st;
     auto part = [&](int n) __attribute__((always_inline)) {
       const int lo = max(ilo - tc * kTile, 0), hi = min(ihi - tc * kTile, kTile - 1);
       if (n < C::LPW) {
@@ -694,12 +714,10 @@ __global__ void __launch_bounds__(256, D == 64 && !FINE ? 2 : 1) win_dkdv_kernel
       }
     };
     constexpr int PARTS = C::LPW + 1;
-    for (int n = 0; n < PARTS; ++n) part(n);
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    // item f + 1 is copied while `step` runs on item f (the last one again, to where nothing reads)
-    auto item = [&](auto step) __attribute__((always_inline)) {
-      if (f + 1 < f1) {
+    // (the last item again, to where nothing reads, when there is no other)
+    auto aim = [&](uint32_t to) __attribute__((always_inline)) {
+      if (fc + 1 < f1) {
+        ++fc;
         ++tc;
         qs += (int64_t)kTile * qrs;
         gs += (int64_t)kTile * grs;
@@ -710,15 +728,37 @@ __global__ void __launch_bounds__(256, D == 64 && !FINE ? 2 : 1) win_dkdv_kernel
           sp += s.TQ;
         }
       }
-      dst = smem_a + ((f + 1 - f0) & 1) * C::STAGE;
-      step(smem_a + ((f - f0) & 1) * C::STAGE);
-      __builtin_amdgcn_s_waitcnt(0);
-      __syncthreads();
+      dst = to;
+    };
+    // the wave's copies have arrived, then everyone's (operands that a step has read ahead are not waited for)
+    auto arrive = [] {
+      __builtin_amdgcn_s_waitcnt(0x0f70);
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    };
+    for (int n = 0; n < PARTS; ++n) part(n);
+    if (AHEAD == 2) {
+      aim(next);
+      for (int n = 0; n < PARTS; ++n) part(n);
+    }
+    arrive();
+    if (AHEAD == 2) wv.prime(st);
+    // item f + AHEAD is copied while `step` runs on item f
+    auto item = [&](auto step) __attribute__((always_inline)) {
+      const uint32_t free_a = AHEAD == 2 ? 3 * lds_at(smem) + 3 * C::STAGE - st - next : next;
+      aim(free_a);
+      step(st, next);
+      arrive();
+      const uint32_t was = st;
+      st = next;
+      next = AHEAD == 2 ? free_a : was;
       ++f;
       ++t;
     };
-    auto idle = [&](uint32_t) {
+    auto idle = [&](uint32_t, uint32_t ahead) {
       for (int n = 0; n < PARTS; ++n) part(n);
+      if (AHEAD == 2) wv.prime(ahead);
     };
     // loops of one form of the step each (a choice inside one loop costs a copy of the sums per tile); every
     // wave passes every item's barrier
@@ -727,11 +767,11 @@ __global__ void __launch_bounds__(256, D == 64 && !FINE ? 2 : 1) win_dkdv_kernel
       while (t < te) {
         while (t < te && (t < tv0 || t >= tv1)) item(idle);
         while (t < min(te, tv1) && (t < tw0 || t >= tw1))
-          item([&](uint32_t st) {
-            wv.template step<true, FINE, PARTS>(st, sq.off + t * kTile + 4 * h - key, lim, part);
+          item([&](uint32_t at, uint32_t ahead) {
+            wv.template step<true, FINE, PARTS>(at, ahead, sq.off + t * kTile + 4 * h - key, lim, part);
           });
         while (t < min(te, tw1) && t >= tw0)
-          item([&](uint32_t st) { wv.template step<false, FINE, PARTS>(st, 0, 0, part); });
+          item([&](uint32_t at, uint32_t ahead) { wv.template step<false, FINE, PARTS>(at, ahead, 0, 0, part); });
       }
       t = tlo;
     }
@@ -771,7 +811,7 @@ __global__ void __launch_bounds__(256, D == 64 && !FINE ? 2 : 1) win_dkdv_kernel
           const float* sp = a.Dsum + stat0 + (size_t)g * s.TQ + i;
           const float p = exp2_hw(fmaf(x, wv.sl, -sp[stats]));
           lost = p != p;
-          const float d = round_bf16(p * (y - sp[0])), pr = round_bf16(p);
+          const float d = round_bf16(p * (y + sp[0])), pr = round_bf16(p);
 #pragma unroll
           for (int dt = 0; dt < C::DT; ++dt)
 #pragma unroll
