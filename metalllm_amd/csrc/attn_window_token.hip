@@ -12,7 +12,7 @@
 //   * V rows are loaded whole (16 lanes x 16 or 8 bytes), the lane's 8 keys of its d chunk, and turned in
 //     registers: one v_perm per pair of values. The d of an output row is E*(4g + r) + e for product e.
 // A step takes 32 keys. Its K registers are loaded again as soon as its scores are formed, its V registers
-// as soon as its products are; the loads of three waves per SIMD cover the rest.
+// as soon as its products are; what one to three waves per SIMD have in flight covers the rest.
 //
 // Split: the steps are dealt to the waves of a workgroup, and over `splits` workgroups where there are
 // too few (sequence, key head) pairs to fill the chip; each part keeps its own reference point and sum, and
@@ -45,6 +45,8 @@ __device__ __forceinline__ bool not_finite(uint32_t pair) {
   return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u;
 }
 
+constexpr int kTokWaves = 4;  // to a workgroup
+
 template <int D>
 struct WtCfg {
   static constexpr int KC = D / 32;  // products over d of a score
@@ -75,12 +77,11 @@ __device__ __forceinline__ WtRange wt_range(const WinShape& s, const WinSeq& q, 
 
 // SEVERAL: more than one query row (TQ > 1), which may see different keys of a step; its path for values that
 // are not finite takes registers that one row does without.
-// WAVES: 4, or 8 where there are so few units that their keys are better split inside one workgroup.
-template <int D, bool SEVERAL, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || SEVERAL ? 2 : D == 64 ? 4 : 3) win_token_kernel(WinFwdArgs a) {
+template <int D, bool SEVERAL>
+__global__ void __launch_bounds__(64 * kTokWaves, SEVERAL ? 2 : D == 64 ? 4 : 3) win_token_kernel(WinFwdArgs a) {
   using C = WtCfg<D>;
-  __shared__ __attribute__((aligned(16))) float sm_o[WAVES][kTokRows][C::PITCH];
-  __shared__ float sm_m[WAVES][kTokRows], sm_l[WAVES][kTokRows];
+  __shared__ __attribute__((aligned(16))) float sm_o[kTokWaves][kTokRows][C::PITCH];
+  __shared__ float sm_m[kTokWaves][kTokRows], sm_l[kTokWaves][kTokRows];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, n16 = lane & 15;
@@ -92,7 +93,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || SEVERAL ? 2 : D == 6
   const WinSeq sq = win_seq(s, b);
   const WtRange w = wt_range(s, sq, rt);
   if (w.i_lo > w.i_hi) return;  // rows behind the sequence: left as they were (the join too)
-  const int parts = WAVES * a.splits, part = WAVES * split + wave;
+  const int parts = kTokWaves * a.splits, part = kTokWaves * split + wave;
   const int t0 = (int)((int64_t)w.steps * part / parts), t1 = (int)((int64_t)w.steps * (part + 1) / parts);
 
   const int row = rt * kTokRows + n16, qi = row / s.G;
@@ -255,12 +256,12 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES == 8 || SEVERAL ? 2 : D == 6
   if (jr >= kTokRows) return;
   float M = -INFINITY;
 #pragma unroll
-  for (int v = 0; v < WAVES; ++v) M = fmaxf(M, sm_m[v][jr]);
+  for (int v = 0; v < kTokWaves; ++v) M = fmaxf(M, sm_m[v][jr]);
   float L = 0.0f, acc[C::E];
 #pragma unroll
   for (int e = 0; e < C::E; ++e) acc[e] = 0.0f;
 #pragma unroll
-  for (int v = 0; v < WAVES; ++v) {
+  for (int v = 0; v < kTokWaves; ++v) {
     const float m = sm_m[v][jr];
     if (m == -INFINITY && sm_l[v][jr] == 0.0f) continue;  // a part without visible keys
     const float f = exp2_hw(m - (M == -INFINITY ? 0.0f : M));
@@ -304,15 +305,16 @@ __global__ void __launch_bounds__(256) win_join_kernel(WinFwdArgs a) {
   const float* in = a.part + ((size_t)unit * a.splits * kTokRows + jr) * (D + 2);
   const size_t step = (size_t)kTokRows * (D + 2);
   float M = -INFINITY;
+#pragma unroll 8
   for (int v = 0; v < a.splits; ++v) M = fmaxf(M, in[v * step + D]);
   const float Mb = M == -INFINITY ? 0.0f : M;
   float L = 0.0f, acc[C::E];
 #pragma unroll
   for (int e = 0; e < C::E; ++e) acc[e] = 0.0f;
-  for (int v = 0; v < a.splits; ++v) {
+#pragma unroll 4
+  for (int v = 0; v < a.splits; ++v) {  // (a part without keys holds m = -inf and zeros)
     const float* p = in + v * step;
     const float m = p[D], l = p[D + 1];
-    if (m == -INFINITY && l == 0.0f) continue;
     const float f = m == -INFINITY ? 1.0f : exp2_hw(m - Mb);
     L = fmaf(l, f, L);
 #pragma unroll
@@ -328,30 +330,29 @@ __global__ void __launch_bounds__(256) win_join_kernel(WinFwdArgs a) {
     a.l[((size_t)b * s.NH + head) * s.TQ + qi] = empty ? -INFINITY : M * (1.0f / kLog2e) + logf(L);
 }
 
-// Waves to a workgroup and workgroups to a unit (sequence, key head, row tile), from the steps that a unit
-// has at most. A workgroup per unit joins its waves in LDS; more of them take a second kernel (about 5 us), so
-// they are for units that are too few to fill the chip and have steps enough for 6 to a wave.
+// Workgroups to a unit (sequence, key head, row tile), from the steps that a unit has at most: as many as put
+// one on each CU, where their waves get 4 steps or more. One workgroup joins its waves in LDS; more take
+// the second kernel. us at (B, TQ, TK, NH, NKV, D), all keys visible but (64, ..), which sees 4096:
+//                                 this   two for each CU  6 steps or more  never split
+//   (4, 1, 4096, 16, 4, 128)      13.2   13.3             16.3             39.8
+//   (16, 1, 4096, 16, 4, 128)     26.4   28.1             26.6             42.9
+//   (64, 1, 8192, 16, 4, 128)     96.8  107.5             96.8             96.8
+// Workgroups of 8 waves, so half as many of them, took 26.0 and 28.7 in the first two.
 static int64_t token_units(const WinShape& s) {
   return (int64_t)s.B * s.NKV * (((int64_t)s.TQ * s.G + kTokRows - 1) / kTokRows);
 }
-static int token_waves(const WinShape& s) { return token_units(s) <= kCus / 2 ? 8 : 4; }
 int win_token_splits(const WinShape& s) {
-  const int64_t units = token_units(s), waves = token_waves(s);
+  const int64_t units = token_units(s);
   const int64_t keys = std::min<int64_t>((int64_t)s.window + s.TQ - 1, s.TK) + s.sinks;
   const int64_t steps = (keys + 31) / 32;
-  const int64_t fill = 12 * kCus / waves;  // workgroups resident at once
-  const int64_t want = std::min<int64_t>((fill + units - 1) / units, steps / (6 * waves));
+  const int64_t want = std::min<int64_t>((kCus + units - 1) / units, steps / (4 * kTokWaves));
   return (int)std::max<int64_t>(1, std::min<int64_t>(want, 64));
 }
 
 template <int D>
 static hipError_t launch_token(const WinFwdArgs& a, unsigned units, hipStream_t s) {
-  const bool several = a.s.TQ > 1;
   const dim3 grid(units * a.splits);
-  if (token_waves(a.s) == 8)
-    hipLaunchKernelGGL((several ? win_token_kernel<D, true, 8> : win_token_kernel<D, false, 8>), grid, dim3(512), 0, s, a);
-  else
-    hipLaunchKernelGGL((several ? win_token_kernel<D, true, 4> : win_token_kernel<D, false, 4>), grid, dim3(256), 0, s, a);
+  hipLaunchKernelGGL((a.s.TQ > 1 ? win_token_kernel<D, true> : win_token_kernel<D, false>), grid, dim3(64 * kTokWaves), 0, s, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
   hipLaunchKernelGGL(win_join_kernel<D>, dim3(units), dim3(256), 0, s, a);
