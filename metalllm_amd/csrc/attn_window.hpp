@@ -119,11 +119,26 @@ __device__ __forceinline__ bool win_sees(const WinShape& s, int pos, int j) {
 }
 
 // ---- host ----
-// Rows of 16 (query row, head of the group) that the single-token form puts into one matrix product, and
-// the largest number of rows per key head that it takes.
+// Which kernel a forward call runs. The one for few rows (attn_window_token.hip) takes tiles of kTokRows rows
+// (query row, head of the group) and splits their keys over the chip; its time is reading the keys once
+// for each tile: units * keys * 4 D bytes at about 6 TB/s. The other (attn_window_fwd.hip) takes blocks of
+// 128 rows of a head, each of which runs along its keys by itself, about 1 us to 64 of them at any
+// number of blocks that run at once. They meet near units * D = 24576. us, few rows' kernel and the other, at
+// (B, TQ, TK, NH, NKV, D), all keys visible:
+//   (1, 32, 16384, 8, 8, 128)    units 16    24   266      (1, 128, 8192, 12, 12, 64)   units 96    44   110
+//   (1, 64, 16384, 32, 8, 128)         128   96   271      (1, 512, 8192, 12, 12, 64)         384   92   110
+//   (4, 32, 4096, 32, 8, 128)          256   83    71      (1, 256, 256, 12, 12, 64)          192  5.6   8.0
+// Up to kTokMost rows of a key head the other one would leave half of its block or more empty: 47 and 77 at
+// (16, 4, 4096, 32, 4, 128), 81 and 77 at (16, 8, ..), 43 and 62 at (16, 8, 4096, 32, 4, 64).
 constexpr int kTokRows = 16;
 constexpr int kTokMost = 64;
-inline bool win_is_token(const WinShape& s) { return s.TQ * s.G <= kTokMost && s.TQ <= kTokRows; }
+constexpr int64_t kTokUnitsD = 24576;
+inline int64_t win_token_units(const WinShape& s) {
+  return (int64_t)s.B * s.NKV * (((int64_t)s.TQ * s.G + kTokRows - 1) / kTokRows);
+}
+inline bool win_is_token(const WinShape& s, int D) {
+  return ((int64_t)s.TQ * s.G <= kTokMost && s.TQ <= kTokRows) || win_token_units(s) * D <= kTokUnitsD;
+}
 int win_token_splits(const WinShape& s);
 inline size_t win_token_floats(const WinShape& s, int D, int splits) {
   const size_t tiles = ((size_t)s.TQ * s.G + kTokRows - 1) / kTokRows;

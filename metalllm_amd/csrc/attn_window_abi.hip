@@ -60,7 +60,7 @@ mla::Span l_span(const metalllmWindowParams& p, const void* t) { return {t, t ? 
 mla::Span len_span(const metalllmWindowParams& p, const void* t) { return {t, t ? 4 * (size_t)p.B : 0}; }
 
 uint64_t forward_bytes(const mla::WinShape& s, int D) {
-  return mla::win_is_token(s) ? 4 * (uint64_t)mla::win_token_floats(s, D, mla::win_token_splits(s)) : 0;
+  return mla::win_is_token(s, D) ? 4 * (uint64_t)mla::win_token_floats(s, D, mla::win_token_splits(s)) : 0;
 }
 // l log2(e) and the row sums of dO * O, each rounded up to whole 16 bytes, then the sink keys' parts
 uint64_t stat_floats(const mla::WinShape& s) { return (2 * (uint64_t)s.B * s.NH * s.TQ + 3) / 4 * 4; }
@@ -110,7 +110,7 @@ int windowAttentionForward(const uint16_t* q, const uint16_t* k, const uint16_t*
       mla::any_overlap({o, ls, ws}))
     return METALLLM_ATTN_E_OVERLAP;
   hipError_t e;
-  if (mla::win_is_token(a.s)) {
+  if (mla::win_is_token(a.s, D)) {
     a.splits = mla::win_token_splits(a.s);
     a.part = (float*)workspace;
     e = mla::launch_window_token(a, D, (hipStream_t)stream);

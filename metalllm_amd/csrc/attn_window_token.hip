@@ -338,11 +338,8 @@ __global__ void __launch_bounds__(256) win_join_kernel(WinFwdArgs a) {
 //   (16, 1, 4096, 16, 4, 128)     26.4   28.1             26.6             42.9
 //   (64, 1, 8192, 16, 4, 128)     96.8  107.5             96.8             96.8
 // Workgroups of 8 waves, so half as many of them, took 26.0 and 28.7 in the first two.
-static int64_t token_units(const WinShape& s) {
-  return (int64_t)s.B * s.NKV * (((int64_t)s.TQ * s.G + kTokRows - 1) / kTokRows);
-}
 int win_token_splits(const WinShape& s) {
-  const int64_t units = token_units(s);
+  const int64_t units = win_token_units(s);
   const int64_t keys = std::min<int64_t>((int64_t)s.window + s.TQ - 1, s.TK) + s.sinks;
   const int64_t steps = (keys + 31) / 32;
   const int64_t want = std::min<int64_t>((kCus + units - 1) / units, steps / (4 * kTokWaves));
@@ -360,7 +357,7 @@ static hipError_t launch_token(const WinFwdArgs& a, unsigned units, hipStream_t 
 }
 
 hipError_t launch_window_token(const WinFwdArgs& a, int D, hipStream_t s) {
-  const unsigned units = (unsigned)token_units(a.s);
+  const unsigned units = (unsigned)win_token_units(a.s);
   return D == 64 ? launch_token<64>(a, units, s) : launch_token<128>(a, units, s);
 }
 

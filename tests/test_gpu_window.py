@@ -23,7 +23,8 @@ TOKENS = [
     C(1, 1, 5000, 2, 1, 128, 5000, 0), C(1, 1, 5000, 3, 1, 64, 4001, 17), C(2, 3, 400, 4, 2, 64, 100, 4),
     C(2, 5, 260, 8, 2, 128, 70, 3, [5, 2], [260, 4]), C(1, 7, 2500, 8, 1, 64, 1500, 40), C(1, 16, 300, 4, 1, 128, 9, 2),
     C(2, 4, 3, 2, 2, 64, 2, 1), C(1, 1, 90, 40, 1, 64, 50, 4), C(1, 1, 150, 72, 1, 64, 60, 4), C(2, 16, 90, 8, 2, 128, 40, 4),
-    C(1, 17, 90, 2, 2, 64, 40, 4), C(300, 1, 40, 2, 1, 64, 20, 2),
+    C(1, 17, 90, 2, 2, 64, 40, 4), C(1, 50, 3000, 6, 2, 64, 2900, 4), C(2, 130, 1500, 4, 1, 128, 1400, 0, [130, 40], [1500, 777]),
+    C(1, 256, 4000, 3, 3, 128, 3800, 7), C(1, 384, 384, 16, 2, 64, 200, 2), C(1, 385, 385, 16, 2, 64, 200, 2), C(300, 1, 40, 2, 1, 64, 20, 2),
 ]
 ROWS = [
     C(1, 17, 17, 1, 1, 64, 100, 0), C(1, 63, 63, 2, 2, 64, 1, 0), C(1, 64, 64, 2, 1, 128, 64, 0),
@@ -88,9 +89,9 @@ def check(c, d, got, want=None):
 
 
 def crowd(c, d, want):
-    """The case again with its sequences repeated to more than 4096 rows in all: a backward pass over fewer takes
-    dS in two parts of bf16."""
-    n = 4096 // (c["B"] * c["NH"] * c["TQ"]) + 1
+    """The case again with its sequences repeated to more than 8192 rows in all: other kernels than those of fewer
+    rows (which split the keys in the forward, and take dS in two parts in the backward)."""
+    n = 8192 // (c["B"] * c["NH"] * c["TQ"]) + 1
     c = dict(c, B=c["B"] * n, **{m: c[m] and c[m] * n for m in ("q_len", "k_len")})
     d = {m: x if x is None else x.repeat(n, *[1] * (x.ndim - 1)) for m, x in d.items()}
     return c, d, {m: tuple(np.concatenate([x] * n) for x in w) for m, w in want.items()}
@@ -122,7 +123,8 @@ def test_gradient_of_few_rows(gpu, c):
 
 
 @pytest.mark.parametrize("layout", ["packed", "token first"])
-@pytest.mark.parametrize("c", [C(2, 150, 150, 4, 2, 64, 40, 5), C(3, 1, 200, 4, 1, 128, 150, 3), C(2, 3, 3, 2, 1, 128, 2, 0)], ids=name_of)
+@pytest.mark.parametrize("c", [C(2, 150, 150, 4, 2, 64, 40, 5), C(3, 1, 200, 4, 1, 128, 150, 3), C(2, 3, 3, 2, 1, 128, 2, 0),
+                               C(3, 1030, 1030, 4, 2, 64, 40, 5), C(2, 700, 900, 8, 2, 128, 50, 0)], ids=name_of)
 def test_strides(gpu, c, layout):
     d = make(c)
     check(c, d, run(c, d, gpu, layout=layout))
@@ -181,7 +183,8 @@ def test_results_repeat(gpu):
         assert torch.equal(a[n], b[n]), n
 
 
-@pytest.mark.parametrize("c", [C(2, 1, 2000, 4, 1, 128, 1500, 4, None, [2000, 900]), C(2, 200, 200, 2, 1, 64, 60, 4)], ids=name_of)
+@pytest.mark.parametrize("c", [C(2, 1, 2000, 4, 1, 128, 1500, 4, None, [2000, 900]), C(2, 200, 200, 2, 1, 64, 60, 4),
+                               C(2, 700, 700, 8, 2, 64, 60, 4)], ids=name_of)
 def test_captured_and_replayed(gpu, c):
     """A captured forward and backward on another stream, replayed with new inputs and lengths."""
     import torch
