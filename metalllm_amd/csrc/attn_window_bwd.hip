@@ -3,19 +3,31 @@
 // With s = q.k/sqrt(D), p = exp(s - l) over the visible keys (l the forward's logsumexp), Dl = sum_d dO.O,
 // dP = dO.v and dS = p (dP - Dl):  dV = P^T.dO,  dK = dS^T.q/sqrt(D),  dQ = dS.k/sqrt(D).
 // Products accumulate in fp32 over all tiles and are rounded once; p and dS are rounded to bf16, the type of
-// the matrix cores' operands (half a step of 2^-8 each, as of the outputs; FINE: dS in two such parts). No atomics: every output has
-// one owner, and the sum over the query heads of a key head runs in the owner, so results repeat bit for bit.
+// the matrix cores' operands (half a step of 2^-8 each, as of the outputs; FINE: dS in two such parts). No
+// atomics: every output has one owner, and the sum over the query heads of a key head runs in the owner, so
+// results repeat bit for bit.
 //
 // Two kernels, then a small one where there are sinks:
 //   win_dq_kernel    query owner: 4 waves x 32 rows of a head, over the key tiles that they see
 //                    (attn_window_fwd.hip's order). Also writes Dl and l log2(e) of its rows for the next.
 //   win_dkdv_kernel  key owner: 4 waves x 32 keys of a key head, over the query tiles that see them, head
 //                    by head of the group. The sinks of block 0 are seen by every later row, so the query
-//                    tiles beyond the block's windows are dealt to workgroups of their own, which keep the
-//                    sums of the sink keys alone in fp32.
+//                    tiles beyond the block's windows are dealt to workgroups of their own, whose waves take
+//                    tiles by themselves for the sums of the sink keys, in fp32.
 //   win_sink_kernel  dK, dV of the sink keys from those parts, in order.
 // A tile that is seen in part is masked by one unsigned compare per score; in the key owner the
-// compare's limit belongs to the lane's key and covers window, sinks and the sequence's end.
+// compare's limit belongs to the lane's key and covers window, sinks and the sequence's end. There the
+// products of dP begin at -Dl, read from LDS where the accumulators have it, which saves a subtraction per
+// score. (In the query owner Dl is the lane's, and 16 registers of it cost more: 135 us against 119 at D = 128.)
+//
+// Bound: instruction issue and, with a full chip, power. A wave's tile of 64 x 32 scores is 1024 cycles of matrix core
+// at D = 64 and 2048 at D = 128 in the key owner, 768 and 1536 in the query owner. The key owner at D = 128 keeps 512
+// registers (its sums alone are 128), so one wave per SIMD, which hides nothing of another's: 409 instructions to
+// 64 products. Measured, each alone: (B, T, NH, NKV, D) = (8, 2048, 12, 12, 64), window 512: 69 and 73 us,
+// 490 and 620 TFLOP/s of visible scores; (2, 4096, 16, 4, 128), window 1024: 114 and 144 us, 790 and 835 TFLOP/s. The
+// sinks' last sums: 5 us.
+// Tried without gain: reads further ahead (4% slower), other paddings of the tiles (a quarter of the LDS cycles are
+// conflicts, but LDS is busy 35% at most), the vector work of two tiles in stages.
 #include "attn_common.hpp"
 #include "attn_window.hpp"
 

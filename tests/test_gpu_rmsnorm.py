@@ -82,7 +82,7 @@ def test_forward_fp8(gpu, rows, cols, group):
     assert (np.abs(value - y) <= tol).all()
 
 
-@pytest.mark.parametrize("rows,cols", SHAPES)
+@pytest.mark.parametrize("rows,cols", SHAPES + [(2049, 104), (2100, 1024), (2048, 1040), (2055, 2040), (513, 2056), (600, 4104)])
 def test_backward(gpu, rows, cols):
     import torch
     import metalllm_amd.rmsnorm as M
