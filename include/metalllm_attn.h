@@ -371,7 +371,7 @@ int metalllmSublayerScratch(const AttentionParams* p, uint64_t need[2], uint64_t
  * some rows see has no part in the others either. A row that sees nothing (lk < lq: pos < 0) gives out = 0,
  * l = -inf, dQ = 0. Elsewhere NaN and infinities spread as the formulas have it.
  * Scores, softmax statistics and sums are fp32; the softmax weights and dS are rounded to bf16 once each as
- * matrix operands, the outputs once at the end. No atomics: results repeat bit for bit.
+ * matrix operands (dS in calls of up to 4096 rows in two parts), the outputs once at the end. No atomics: results repeat bit for bit.
  * Workspace: the size functions' bytes (0 possible for the forward: workspace may then be NULL), 16-byte
  * aligned, no state between calls; it belongs to one call (or captured call's replay) at a time. The sizes
  * depend on the params alone. Nothing is allocated and no memset is recorded: every call can be captured.
