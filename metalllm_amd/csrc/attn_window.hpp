@@ -49,6 +49,7 @@ struct WinBwdArgs {
   float* Dsum;  // [B, NH, TQ] workspace, twice: -Dl (Dl = sum over d of dO O), l log2(e)
   float* part;  // workspace: partial dK, dV of the sink keys, or NULL where nothing is split (splits = 0)
   int splits;
+  bool narrow;  // win_is_narrow
 };
 
 // A sequence's lengths, held inside the buffers whatever the device arrays say.
@@ -153,6 +154,16 @@ inline int win_sink_splits(const WinShape& s) {
   const int64_t n = (s.G * ((far + kTile - 1) / kTile) + 7) / 8, groups = (int64_t)s.B * s.NKV;
   const int64_t most = 4096 / groups < 8 ? 8 : 4096 / groups < 128 ? 4096 / groups : 128;
   return (int)(n < most ? n : most);
+}
+// Backward with key blocks for a quarter of the CUs or fewer and four query tiles or more to each: blocks of 32
+// keys, whose waves take tiles each by itself and join their sums in LDS. Whole backward, us, with blocks of 32
+// and of 128, at (B, T, NH, NKV, D), every key visible: (1, 4096, 8, 2, 128) 280, 458; (1, 521, 12, 3, 128) 58, 82;
+// (2, 1024, 12, 4, 128) 75, 104; two tiles, (1, 100, 4, 4, 64), 20.5, 19.2. Not with far rows of sinks, which block 0
+// would take alone: (1, 4096, 4, 2, 64), window 256, 74, 37.
+inline bool win_is_narrow(const WinShape& s) {
+  const int64_t blocks = (int64_t)s.B * s.NKV * ((s.TK + kBwdBlockN - 1) / kBwdBlockN);
+  const int64_t rows = s.TQ < (int64_t)s.window + kBwdBlockN - 1 ? s.TQ : (int64_t)s.window + kBwdBlockN - 1;
+  return blocks <= kCus / 4 && s.G * ((rows + kTile - 1) / kTile) >= 4 && win_sink_splits(s) == 0;
 }
 inline size_t win_sink_floats(const WinShape& s, int D, int splits) {  // [group][part][dK, dV][sink][D]
   return splits ? (size_t)s.B * s.NKV * (splits + 1) * 2 * s.sinks * D : 0;

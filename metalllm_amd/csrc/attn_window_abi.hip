@@ -131,8 +131,9 @@ int windowAttentionBackward(const uint16_t* dO, const uint16_t* O, const float* 
                         (const void*)dQ, (const void*)dK, (const void*)dV, (const void*)workspace})
     if (!aligned(t, 16)) return METALLLM_ATTN_E_ALIGN;
   if (!aligned(q_len, 4) || !aligned(k_len, 4)) return METALLLM_ATTN_E_ALIGN;
-  mla::WinBwdArgs a{dO, O, l, q, k, v, dQ, dK, dV, shape_of(*p, q_len, k_len), (float*)workspace, nullptr, 0};
+  mla::WinBwdArgs a{dO, O, l, q, k, v, dQ, dK, dV, shape_of(*p, q_len, k_len), (float*)workspace, nullptr, 0, false};
   const int D = (int)p->D;
+  a.narrow = mla::win_is_narrow(a.s);
   if (workspace_bytes < backward_bytes(a.s, D)) return METALLLM_ATTN_E_SIZE;
   // dQ, dK and dV may be interleaved with each other (slices of one buffer), not with anything read
   const mla::Span ws{workspace, (size_t)backward_bytes(a.s, D)};

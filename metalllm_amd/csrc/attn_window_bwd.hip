@@ -598,12 +598,13 @@ struct WinKeyWave {
 template <int D, bool FINE>
 __global__ void __launch_bounds__(256, D == 64 && !FINE ? 2 : 1) win_dkdv_kernel(WinBwdArgs a) {
   using C = WbCfg<D>;
-  constexpr int BN = kBwdBlockN;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * C::STAGE];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int h = lane >> 5, l32 = lane & 31;
   const WinShape& s = a.s;
+  const bool narrow = a.narrow;  // blocks of 32 keys
+  const int BN = narrow ? 32 : kBwdBlockN;
   const int nkb = (s.TK + BN - 1) / BN;
   // the key blocks first, then (far) the parts of the rows that see block 0's sinks alone
   const int groups = s.B * s.NKV, near = groups * nkb;
@@ -625,6 +626,7 @@ __global__ void __launch_bounds__(256, D == 64 && !FINE ? 2 : 1) win_dkdv_kernel
   int ilo = max(0, k0 - sq.off);
   int ihi = min(sq.lq - 1, min(k1 + s.window - 1, sq.lk - 1) - sq.off);
   int tlo = 0, nt = 0;
+  if (narrow && k0 < s.sinks) ihi = sq.lq - 1;
   if (ilo <= ihi) {
     tlo = ilo / kTile;
     nt = ihi / kTile - tlo + 1;
@@ -644,9 +646,10 @@ __global__ void __launch_bounds__(256, D == 64 && !FINE ? 2 : 1) win_dkdv_kernel
   const int f0 = far ? (int)((int64_t)items * blk / a.splits) : 0;
   const int f1 = far ? (int)((int64_t)items * (blk + 1) / a.splits) : items;
 
-  // far: a wave takes every fs-th item alone, for 32 sinks
-  const int halves = far ? (s.sinks + 31) / 32 : 1, fs = far ? 4 / halves : 1, fw = far ? f0 + wave / halves : f0;
-  const int kw0 = far ? 32 * (wave % halves) : k0 + 32 * wave, kw1 = min(kw0 + 31, k1);
+  // alone: a wave takes every fs-th item by itself, for 32 sinks (far) or the block's 32 keys (narrow)
+  const bool alone = far || narrow;
+  const int halves = far ? (s.sinks + 31) / 32 : 1, fs = alone ? 4 / halves : 1, fw = alone ? f0 + wave / halves : f0;
+  const int kw0 = far ? 32 * (wave % halves) : narrow ? k0 : k0 + 32 * wave, kw1 = min(kw0 + 31, k1);
   const int key = kw0 + l32;
   const bool sink_key = key < s.sinks;
   const int most = sq.lk - key;  // rows of the sequence that stand at the key or behind it
@@ -681,7 +684,7 @@ __global__ void __launch_bounds__(256, D == 64 && !FINE ? 2 : 1) win_dkdv_kernel
   tw1 = min(tw1, tv1);
   if (tw0 >= tw1) tw0 = tw1 = tv1;
 
-  if (far) {
+  if (alone) {
     const uint32_t st = lds_at(smem) + wave * C::STAGE;
     for (int f = fw; f < f1; f += fs) {
       const int g = f / nt, t = tlo + f - g * nt;
@@ -789,7 +792,7 @@ __global__ void __launch_bounds__(256, D == 64 && !FINE ? 2 : 1) win_dkdv_kernel
     }
   }
 
-  if (!wave_on && !far) return;
+  if (!wave_on && !alone) return;
   // A row that does not see a key but shares its tile adds 0 * NaN to it where q or dO is not finite: such
   // keys are summed again over the rows that see them.
   float bad = 0.0f;
@@ -846,19 +849,19 @@ __global__ void __launch_bounds__(256, D == 64 && !FINE ? 2 : 1) win_dkdv_kernel
     }
   }
   const uint32_t lds = lds_at(smem) + wave * kRowsOut<D>;  // (every wave is past its last item)
-  if (!far) {
+  if (!alone) {
     auto live = [&](int r) { return kw0 + r <= k1 && !(split && kw0 + r < s.sinks); };
     store_rows<D>(lds, lane, wv.st + C::DT, s.scale, a.dK + b * s.k_seq + (size_t)kw0 * s.k_row + kvh * D, s.k_row, live);
     store_rows<D>(lds, lane, wv.st, 1.0f, a.dV + b * s.v_seq + (size_t)kw0 * s.v_row + kvh * D, s.v_row, live);
   }
-  if (!split) return;
-  // sums of the sinks, fp32 [dK, dV][sink][D]: part 0 the block's own rows, then the far parts, whose waves
-  // join theirs in LDS
+  if (!split && !narrow) return;
+  // sums of the sinks, fp32 [dK, dV][sink][D]: part 0 the block's own rows, then the far parts; waves that took
+  // items alone join their sums in LDS
   float* out = a.part + ((size_t)group * (a.splits + 1) + (far ? blk + 1 : 0)) * 2 * s.sinks * D;
   float* own = (float*)(smem + wave * C::STAGE);
-  float *ko = far ? own + l32 * 2 * D : out + key * D, *vo = far ? ko + D : ko + s.sinks * D;
+  float *ko = alone ? own + l32 * 2 * D : out + key * D, *vo = alone ? ko + D : ko + s.sinks * D;
   static_assert(32 * 2 * D * 4 <= C::STAGE, "a wave's sums in its stage");
-  if (sink_key && key <= k1)
+  if ((sink_key || narrow) && key <= k1)
 #pragma unroll
     for (int dt = 0; dt < C::DT; ++dt)
 #pragma unroll
@@ -869,13 +872,20 @@ __global__ void __launch_bounds__(256, D == 64 && !FINE ? 2 : 1) win_dkdv_kernel
         *(f32x4*)(ko + d0) = f32x4{k[4 * u], k[4 * u + 1], k[4 * u + 2], k[4 * u + 3]};
         *(f32x4*)(vo + d0) = f32x4{v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]};
       }
-  if (!far) return;
+  if (!alone) return;
   __syncthreads();
-  for (int n = tid; n < min(s.sinks, sq.lk) * (D / 2); n += 256) {
+  for (int n = tid; n < (narrow ? k1 - k0 + 1 : min(s.sinks, sq.lk)) * (D / 2); n += 256) {
     const int j = n / (D / 2), c = 4 * (n % (D / 2));
     f32x4 sum = {0, 0, 0, 0};
     for (int w = j / 32; w < 4; w += halves) sum += *(const f32x4*)(smem + w * C::STAGE + 4 * ((j & 31) * 2 * D + c));
-    *(f32x4*)(out + (c < D ? j * D + c : (s.sinks + j) * D + c - D)) = sum;
+    if (!narrow) {
+      *(f32x4*)(out + (c < D ? j * D + c : (s.sinks + j) * D + c - D)) = sum;
+      continue;
+    }
+    if (c < D) sum *= s.scale;
+    uint16_t* o = c < D ? a.dK + b * s.k_seq + (size_t)(k0 + j) * s.k_row + c
+                        : a.dV + b * s.v_seq + (size_t)(k0 + j) * s.v_row + c - D;
+    *(u32x2*)(o + kvh * D) = u32x2{pack_bf16(sum[0], sum[1]), pack_bf16(sum[2], sum[3])};
   }
 }
 
@@ -909,7 +919,7 @@ hipError_t launch(const WinBwdArgs& a, hipStream_t s) {
   const WinShape& p = a.s;
   const unsigned groups = (unsigned)(p.B * p.NKV);
   const unsigned nq = groups * p.G * ((p.TQ + kDqBlockM - 1) / kDqBlockM);
-  const unsigned nk = groups * ((p.TK + kBwdBlockN - 1) / kBwdBlockN + a.splits);
+  const unsigned nk = a.narrow ? groups * ((p.TK + 31) / 32) : groups * ((p.TK + kBwdBlockN - 1) / kBwdBlockN + a.splits);
   hipLaunchKernelGGL((win_dq_kernel<D, FINE>), dim3(nq), dim3(256), 0, s, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
